@@ -279,6 +279,114 @@ int sampler_batched_noalloc(const SamplerBatchConfig* cfg, const float* logits, 
                             void* stream);
 
 /* ------------------------------------------------------------------------
+ * Filtered sampling and the 8-bit classifier (no counterpart in the
+ * reference, whose sampler knows temperature and top-p over fp32 logits and
+ * whose classifier is fp32 or 16-bit).  Device buffers; every call is
+ * asynchronous on `stream` and can be captured into a CUDA graph.
+ * ---------------------------------------------------------------------- */
+
+/* Element types of the 16- and 32-bit buffers below. */
+#define SAMPLER_DTYPE_F32 0
+#define SAMPLER_DTYPE_BF16 1
+#define SAMPLER_DTYPE_F16 2
+
+/* Largest vocabulary sampler_filtered accepts. */
+#define SAMPLER_FILTERED_MAX_VOCAB 1048576
+
+typedef struct {
+    int vocab_size;    /* V, 1 <= V <= SAMPLER_FILTERED_MAX_VOCAB */
+    int logits_dtype;  /* SAMPLER_DTYPE_* */
+    float temperature; /* each of the four: for every row unless its per-row array is given */
+    int topk;          /* <= 0: off */
+    float topp;        /* <= 0, >= 1 or NaN: off */
+    float minp;        /* <= 0 or NaN: off; above 1 counts as 1 */
+} SamplerFilterConfig;
+
+/* Samples `batch` rows by temperature, top-k, top-p and min-p with one random
+ * number per row.  The entries of a row above -infinity are its candidates,
+ * ordered by falling logit, ties by rising index; entry i has the weight
+ * w_i = exp((l_i - max l) / T), and the filters keep a prefix of the order:
+ *   n1 = the candidates, of these the first topk, of these those with w_i >= minp
+ *   n  = the shortest prefix whose mass exceeds topp * (mass of the n1), or n1
+ * The token is the first of the n whose running mass exceeds
+ * coin * (mass of the n).  A row with T < 1e-6 (zero, negative and NaN ones
+ * included) takes its first candidate (n = 1) and draws no coin.
+ *   logits           [batch, ld] of logits_dtype, row r at logits + r*ld (any
+ *                    ld >= V, any element alignment; read only).  A NaN is no
+ *                    candidate and flags its row SAMPLER_ROW_NAN; several
+ *                    +infinity entries share the whole mass
+ *   *_rows           [batch] or NULL (then the config's value)
+ *   coins            [batch] or NULL: given coins, clamped to [0, 1 - 2^-24]
+ *                    (NaN: 0), instead of a draw from rng_state
+ *   rng_state        [batch] xorshift states, advanced by one draw on rows
+ *                    with T >= 1e-6 (neither read nor written with coins)
+ *   out_ids          [batch] token ids; 0 on a row without candidates, which is
+ *                    flagged SAMPLER_ROW_NO_CANDIDATE
+ *   out_logprobs     [batch] or NULL: ln(w_id / mass of the n); -infinity
+ *                    without candidates
+ *   out_kept         [batch] or NULL: n
+ *   row_flags        [batch] or NULL: SAMPLER_ROW_NAN, SAMPLER_ROW_NO_CANDIDATE
+ * Weights and sums that decide an id are held to about 2^-43 of the largest
+ * weight, so ids are those of real arithmetic up to that and do not depend on
+ * scheduling.  With the same coin it draws as sampler_batched does when that
+ * row takes sample_topp; with top-p off, sampler_batched walks in index order
+ * (sample_mult) and this call in falling order.  No workspace, no library
+ * buffers: calls on different streams may overlap. */
+int sampler_filtered(const SamplerFilterConfig* cfg, const void* logits, int batch, long long ld,
+                     const float* temperature_rows, const int* topk_rows, const float* topp_rows,
+                     const float* minp_rows, const float* coins, unsigned long long* rng_state, int* out_ids,
+                     float* out_logprobs, int* out_kept, int* row_flags, void* stream);
+
+/* x [rows, dim] (row r at x + r*ld, SAMPLER_DTYPE_*) as float8 e4m3 with one
+ * fp32 scale per block of block_rows (1: activations, 128: weights) by 128
+ * columns, the last blocks shorter where rows or dim end:
+ *   s = max(amax / 448, 2^-126),  q = e4m3(x / s)   (nearest, ties to even)
+ * A block holding a NaN or an infinity gets scale NaN and NaN values.
+ *   out_q      [rows, dim] bytes, contiguous
+ *   out_scales [ceil(rows / block_rows), ceil(dim / 128)] */
+int quantize_fp8(const void* x, int x_dtype, int rows, int dim, long long ld, int block_rows, void* out_q,
+                 float* out_scales, void* stream);
+
+/* The final RMSNorm (as rmsnorm_bf16, of rows in fp32 or 16 bits) and
+ * quantize_fp8 of its fp32 result at block_rows 1, in one pass. */
+int rmsnorm_fp8(const void* x, int x_dtype, const float* norm_weight, int batch, int dim, long long ld, void* out_q,
+                float* out_scales, void* stream);
+
+/* The classifier projection from 8-bit operands, fp32 accumulation:
+ *   logits[b, v] = sum over blocks g of 128 columns of
+ *                  hidden_scales[b, g] * wcls_scales[v / 128, g] * sum_{k in g} hidden[b, k] * wcls[v, k]
+ *   hidden, hidden_scales   as quantize_fp8 at block_rows 1 or rmsnorm_fp8 write them: e4m3 [batch, dim]
+ *   wcls, wcls_scales       as quantize_fp8 at block_rows 128 writes them: e4m3 [vocab, dim]
+ *   logits_out              [batch, ld], SAMPLER_DTYPE_F32 or _BF16, ld >= vocab (what lies between the
+ *                           rows stays as it is)
+ * dim % 16 == 0, dim <= 65536; hidden and wcls 16-byte aligned; any vocab.  The product of two scales
+ * has to be a finite fp32 number. */
+int classifier_logits_fp8(const void* hidden, const float* hidden_scales, const void* wcls, const float* wcls_scales,
+                          int batch, int dim, int vocab, void* logits_out, int logits_dtype, long long ld,
+                          void* stream);
+
+/* Bytes of workspace classifier_fp8_sample_filtered needs; logits_dtype < 0
+ * when the call gets a logits_out. */
+size_t classifier_fp8_workspace_bytes(int batch, int dim, int vocab, int logits_dtype);
+
+/* The decode step on 8-bit weights from the last layer's output: rmsnorm_fp8
+ * (quantize_fp8 when norm_weight is NULL) of x [batch, dim], contiguous,
+ * classifier_logits_fp8, then sampler_filtered over its logits (cfg->logits_dtype:
+ * SAMPLER_DTYPE_F32 or _BF16, the type the logits are rounded to).
+ *   logits_out  [batch, vocab_size] of that type, or NULL (then in the workspace)
+ *   workspace   a device buffer of classifier_fp8_workspace_bytes(), 16-byte
+ *               aligned, for the 8-bit operand and the logits; the caller's, so
+ *               that calls which may overlap, and graphs whose replays may, have
+ *               one each */
+int classifier_fp8_sample_filtered(const SamplerFilterConfig* cfg, const void* x, int x_dtype,
+                                   const float* norm_weight, const void* wcls, const float* wcls_scales, int batch,
+                                   int dim, const float* temperature_rows, const int* topk_rows,
+                                   const float* topp_rows, const float* minp_rows, const float* coins,
+                                   unsigned long long* rng_state, int* out_ids, float* out_logprobs, int* out_kept,
+                                   void* logits_out, int* row_flags, void* workspace, size_t workspace_bytes,
+                                   void* stream);
+
+/* ------------------------------------------------------------------------
  * Multi-GPU helpers (no counterpart in the reference, which is single-GPU:
  * llama2_cublas.cu:6065 calls cudaSetDevice(0)).
  * ---------------------------------------------------------------------- */

@@ -19,6 +19,8 @@ MODE_DO_SAMPLE = SAMPLER_FLAG_GREEDY_BELOW_1E6
 MODE_SAMPLE_DEBUG = SAMPLER_FLAG_GREEDY_BELOW_1E6 | SAMPLER_FLAG_NAN_TOKEN1
 ROW_NAN, ROW_NO_CANDIDATE, ROW_SLOW_PATH, ROW_SERIAL, ROW_TIMEOUT = 1, 2, 4, 8, 16
 MAX_VOCAB = 32768
+DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
+FILTERED_MAX_VOCAB = 1048576
 
 # Every symbol the header declares (the CPU tests check the library exports them).
 EXPORTED_SYMBOLS = [
@@ -28,7 +30,8 @@ EXPORTED_SYMBOLS = [
     "sampler_nccl_get_unique_id", "sampler_nccl_comm_init", "sampler_nccl_allgather_ids",
     "sampler_nccl_comm_destroy", "sampler_batched_noalloc", "classifier_sample_fused",
     "classifier_logits", "rmsnorm_bf16", "classifier_rmsnorm_sample_fused", "sampler_gather_rows",
-    "sampler_selftest_wait_timeout",
+    "sampler_selftest_wait_timeout", "sampler_filtered", "quantize_fp8", "rmsnorm_fp8", "classifier_logits_fp8",
+    "classifier_fp8_workspace_bytes", "classifier_fp8_sample_filtered",
 ]
 
 
@@ -50,6 +53,11 @@ class Sampler(ctypes.Structure):
 class SamplerBatchConfig(ctypes.Structure):
     _fields_ = [("vocab_size", ctypes.c_int), ("temperature", ctypes.c_float),
                 ("topp", ctypes.c_float), ("flags", ctypes.c_int)]
+
+
+class SamplerFilterConfig(ctypes.Structure):
+    _fields_ = [("vocab_size", ctypes.c_int), ("logits_dtype", ctypes.c_int), ("temperature", ctypes.c_float),
+                ("topk", ctypes.c_int), ("topp", ctypes.c_float), ("minp", ctypes.c_float)]
 
 
 _lib = None
@@ -126,6 +134,20 @@ def lib():
     L.sampler_gather_rows.restype = c_int
     L.sampler_selftest_wait_timeout.argtypes = [ctypes.c_uint, ctypes.POINTER(c_int)]
     L.sampler_selftest_wait_timeout.restype = c_int
+    c_ll = ctypes.c_longlong
+    L.sampler_filtered.argtypes = [ctypes.POINTER(SamplerFilterConfig), P, c_int, c_ll, P, P, P, P, P, P, P, P, P, P, P]
+    L.sampler_filtered.restype = c_int
+    L.quantize_fp8.argtypes = [P, c_int, c_int, c_int, c_ll, c_int, P, P, P]
+    L.quantize_fp8.restype = c_int
+    L.rmsnorm_fp8.argtypes = [P, c_int, P, c_int, c_int, c_ll, P, P, P]
+    L.rmsnorm_fp8.restype = c_int
+    L.classifier_logits_fp8.argtypes = [P, P, P, P, c_int, c_int, c_int, P, c_int, c_ll, P]
+    L.classifier_logits_fp8.restype = c_int
+    L.classifier_fp8_workspace_bytes.argtypes = [c_int, c_int, c_int, c_int]
+    L.classifier_fp8_workspace_bytes.restype = c_size
+    L.classifier_fp8_sample_filtered.argtypes = [ctypes.POINTER(SamplerFilterConfig), P, c_int, P, P, P, c_int, c_int,
+                                                 P, P, P, P, P, P, P, P, P, P, P, P, c_size, P]
+    L.classifier_fp8_sample_filtered.restype = c_int
     _lib = L
     return L
 
@@ -292,6 +314,206 @@ def sample_batched_host(logits_np, temperature, topp, states_np, topp_rows_np=No
                                     ids.ctypes.data_as(ctypes.c_void_p))
     _check(rc, "sampler_batched_host")
     return ids
+
+
+# ---- filtered sampling and the 8-bit classifier ----
+_DTYPE_CODES = {}
+
+
+def _dtype_code(t, what):
+    if not _DTYPE_CODES:
+        import torch
+        _DTYPE_CODES.update({torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16})
+    code = _DTYPE_CODES.get(t.dtype)
+    if code is None:
+        raise SamplerError(f"{what} must be float32, bfloat16 or float16, not {t.dtype}")
+    return code
+
+
+def _vector(t, what, n, dtype, device):
+    """Address of a contiguous vector of n elements on `device`; None passes."""
+    if t is None:
+        return None
+    if t.dtype != dtype or t.numel() != n or not t.is_contiguous() or t.device != device:
+        raise SamplerError(f"{what} must be a contiguous {dtype} tensor of {n} elements on {device}")
+    return t.data_ptr()
+
+
+def _matrix(t, what):
+    """Checks a row-major [R, C] CUDA tensor (any row stride that keeps rows apart)."""
+    if t.dim() != 2 or not t.is_cuda or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise SamplerError(f"{what} must be a row-major CUDA matrix")
+    if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        raise SamplerError(f"{what} has overlapping rows")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _block_matrix(t, what, shape, dtype, device):
+    if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous() or t.device != device:
+        raise SamplerError(f"{what} must be a contiguous {dtype} tensor {list(shape)} on {device}")
+    return t.data_ptr()
+
+
+def _on_device(device, rows, stream, fn, *args):
+    """fn(*args, stream) with the operands' device current, on `stream`
+    (default: that device's current one); nothing for an empty batch, whose
+    tensors have no address."""
+    import torch
+    if rows == 0:
+        return
+    if torch.cuda.current_device() != device.index:
+        with torch.cuda.device(device):
+            return _on_device(device, rows, stream, fn, *args)
+    if stream is None:
+        stream = torch.cuda.current_stream()
+    elif stream.device != device:
+        raise SamplerError(f"the stream is on {stream.device}, the operands on {device}")
+    rc = fn(*args, stream.cuda_stream)
+    if rc != 0:
+        _check(rc, fn.__name__)
+
+
+def _filter_rows(B, dev, temperature_rows, topk_rows, topp_rows, minp_rows, coins, rng_state):
+    import torch
+    f32 = torch.float32
+    return (_vector(temperature_rows, "temperature_rows", B, f32, dev),
+            _vector(topk_rows, "topk_rows", B, torch.int32, dev), _vector(topp_rows, "topp_rows", B, f32, dev),
+            _vector(minp_rows, "minp_rows", B, f32, dev), _vector(coins, "coins", B, f32, dev),
+            _vector(rng_state, "rng_state", B, torch.int64, dev))
+
+
+def sample_filtered(logits, temperature, topk, topp, minp, rng_state=None, *, temperature_rows=None, topk_rows=None,
+                    topp_rows=None, minp_rows=None, coins=None, out_ids=None, logprobs_out=None, kept_out=None,
+                    row_flags=None, stream=None):
+    """Token ids of the rows of a CUDA float32, bfloat16 or float16 matrix
+    [B, V] (any row stride, V up to FILTERED_MAX_VOCAB) by temperature, top-k,
+    top-p and min-p, each for every row or per row (*_rows; top-k int32), from
+    given coins or one draw of rng_state per row.  topk <= 0, topp outside
+    (0, 1) and minp <= 0 are off; a row with T < 1e-6 takes its first largest
+    logit.  logprobs_out float32, kept_out and row_flags int32 (each [B])
+    receive ln(p) of the id among the kept entries, their count, and the row's
+    ROW_* bits.  Returns out_ids (int32 CUDA tensor [B]).  Asynchronous on
+    `stream`."""
+    import torch
+    ld = _matrix(logits, "logits")
+    B, V = logits.shape
+    dev = logits.device
+    if out_ids is None:
+        out_ids = torch.empty(B, dtype=torch.int32, device=dev)
+    i32 = torch.int32
+    cfg = SamplerFilterConfig(V, _dtype_code(logits, "logits"), temperature, topk, topp, minp)
+    _on_device(dev, B, stream, lib().sampler_filtered, ctypes.byref(cfg), logits.data_ptr(), B, ld,
+               *_filter_rows(B, dev, temperature_rows, topk_rows, topp_rows, minp_rows, coins, rng_state),
+               _vector(out_ids, "out_ids", B, i32, dev), _vector(logprobs_out, "logprobs_out", B, torch.float32, dev),
+               _vector(kept_out, "kept_out", B, i32, dev), _vector(row_flags, "row_flags", B, i32, dev))
+    return out_ids
+
+
+def _fp8_outputs(x, block_rows, out, scales_out):
+    import torch
+    R, D = x.shape
+    shape = (-(-R // block_rows), -(-D // 128))
+    if out is None:
+        out = torch.empty(R, D, dtype=torch.float8_e4m3fn, device=x.device)
+    if scales_out is None:
+        scales_out = torch.empty(shape, dtype=torch.float32, device=x.device)
+    return (out, scales_out, _block_matrix(out, "out", (R, D), torch.float8_e4m3fn, x.device),
+            _block_matrix(scales_out, "scales_out", shape, torch.float32, x.device))
+
+
+def quantize_fp8(x, block_rows=1, *, out=None, scales_out=None, stream=None):
+    """x (float32, bfloat16 or float16 CUDA matrix [R, D], any row stride) as
+    float8_e4m3fn [R, D] with one float32 scale per block of block_rows (1 for
+    activations, 128 for weights) by 128 columns.  Returns (values, scales)."""
+    ld = _matrix(x, "x")
+    if block_rows not in (1, 128):
+        raise SamplerError("block_rows must be 1 or 128")
+    out, scales_out, qp, sp = _fp8_outputs(x, block_rows, out, scales_out)
+    _on_device(x.device, x.shape[0], stream, lib().quantize_fp8, x.data_ptr(), _dtype_code(x, "x"), x.shape[0], x.shape[1], ld,
+               block_rows, qp, sp)
+    return out, scales_out
+
+
+def rmsnorm_fp8(x, norm_weight, *, out=None, scales_out=None, stream=None):
+    """quantize_fp8(norm_weight * x / rms(x)) with block_rows 1 in one pass: x
+    float32, bfloat16 or float16 [B, D], norm_weight float32 [D]."""
+    import torch
+    ld = _matrix(x, "x")
+    out, scales_out, qp, sp = _fp8_outputs(x, 1, out, scales_out)
+    wp = _vector(norm_weight, "norm_weight", x.shape[1], torch.float32, x.device)
+    _on_device(x.device, x.shape[0], stream, lib().rmsnorm_fp8, x.data_ptr(), _dtype_code(x, "x"), wp, x.shape[0], x.shape[1], ld,
+               qp, sp)
+    return out, scales_out
+
+
+def _fp8_weights(wcls, wcls_scales, D, dev):
+    import torch
+    if wcls.dim() != 2 or wcls.shape[1] != D:
+        raise SamplerError(f"wcls must be [V, {D}]")
+    V = wcls.shape[0]
+    return (V, _block_matrix(wcls, "wcls", (V, D), torch.float8_e4m3fn, dev),
+            _block_matrix(wcls_scales, "wcls_scales", (-(-V // 128), -(-D // 128)), torch.float32, dev))
+
+
+def classifier_logits_fp8(hidden, hidden_scales, wcls, wcls_scales, logits_out=None, stream=None):
+    """logits = (hidden * hidden_scales) . (wcls * wcls_scales)^T with fp32
+    accumulation, from quantize_fp8's operands (hidden at block_rows 1 or
+    rmsnorm_fp8's, wcls at 128).  logits_out: float32 (default) or bfloat16
+    [B, V], any row stride."""
+    import torch
+    if hidden.dim() != 2 or not hidden.is_cuda:
+        raise SamplerError("hidden must be a CUDA matrix")
+    B, D = hidden.shape
+    dev = hidden.device
+    hp = _block_matrix(hidden, "hidden", (B, D), torch.float8_e4m3fn, dev)
+    hsp = _block_matrix(hidden_scales, "hidden_scales", (B, -(-D // 128)), torch.float32, dev)
+    V, wp, wsp = _fp8_weights(wcls, wcls_scales, D, dev)
+    if logits_out is None:
+        logits_out = torch.empty(B, V, dtype=torch.float32, device=dev)
+    ld = _matrix(logits_out, "logits_out")
+    if tuple(logits_out.shape) != (B, V) or logits_out.device != dev:
+        raise SamplerError(f"logits_out must be [{B}, {V}] on {dev}")
+    _on_device(dev, B, stream, lib().classifier_logits_fp8, hp, hsp, wp, wsp, B, D, V, logits_out.data_ptr(),
+               _dtype_code(logits_out, "logits_out"), ld)
+    return logits_out
+
+
+def classifier_fp8_sample_filtered(x, norm_weight, wcls, wcls_scales, temperature, topk, topp, minp, rng_state=None,
+                                   *, temperature_rows=None, topk_rows=None, topp_rows=None, minp_rows=None,
+                                   coins=None, out_ids=None, logprobs_out=None, kept_out=None, logits_out=None,
+                                   row_flags=None, stream=None):
+    """Decode step on 8-bit weights from hidden states x [B, D] (contiguous
+    float32, bfloat16 or float16): rmsnorm_fp8 (quantize_fp8 when norm_weight
+    is None), classifier_logits_fp8, sample_filtered.  logits_out: contiguous
+    float32 or bfloat16 [B, V] that receives the logits (float32 otherwise).
+    Returns out_ids."""
+    import torch
+    if x.dim() != 2 or not x.is_cuda or not x.is_contiguous():
+        raise SamplerError("x must be a contiguous CUDA matrix")
+    B, D = x.shape
+    dev = x.device
+    V, wp, wsp = _fp8_weights(wcls, wcls_scales, D, dev)
+    code, lp = DTYPE_F32, None
+    if logits_out is not None:
+        code = _dtype_code(logits_out, "logits_out")
+        lp = _block_matrix(logits_out, "logits_out", (B, V), logits_out.dtype, dev)
+    L = lib()
+    n = L.classifier_fp8_workspace_bytes(B, D, V, code if lp is None else -1)
+    # from torch's allocator: ordered on the stream, and a graph's own inside a capture
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    if stream is not None:
+        ws.record_stream(stream)
+    if out_ids is None:
+        out_ids = torch.empty(B, dtype=torch.int32, device=dev)
+    i32 = torch.int32
+    cfg = SamplerFilterConfig(V, code, temperature, topk, topp, minp)
+    _on_device(dev, B, stream, L.classifier_fp8_sample_filtered, ctypes.byref(cfg), x.data_ptr(), _dtype_code(x, "x"),
+               _vector(norm_weight, "norm_weight", D, torch.float32, dev), wp, wsp, B, D,
+               *_filter_rows(B, dev, temperature_rows, topk_rows, topp_rows, minp_rows, coins, rng_state),
+               _vector(out_ids, "out_ids", B, i32, dev), _vector(logprobs_out, "logprobs_out", B, torch.float32, dev),
+               _vector(kept_out, "kept_out", B, i32, dev), lp, _vector(row_flags, "row_flags", B, i32, dev),
+               ws.data_ptr(), n)
+    return out_ids
 
 
 def last_launch_count():

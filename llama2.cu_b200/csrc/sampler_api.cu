@@ -6,6 +6,7 @@
 // device or the kernels are unavailable, calls fail (-1 / SAMPLER_E_*) with a
 // message in sampler_last_error().
 #include "../../include/b200_sampler.h"
+#include "fp8_filter_kernels.cuh"
 #include "sampler_kernels.cuh"
 
 #include <cuda_runtime.h>
@@ -701,6 +702,214 @@ int classifier_logits(const void* hidden, const void* wcls, int batch, int dim, 
     if (n < 0) return fail(SAMPLER_E_CUDA, "classifier GEMM launch: %s", cudaGetErrorString((cudaError_t)(-n)));
     g_last_launches = n;
     return SAMPLER_OK;
+}
+
+}  // extern "C"
+
+// ===========================================================================
+// Filtered sampling and the 8-bit classifier
+// ===========================================================================
+namespace {
+constexpr int kMaxDim = 1 << 24;      // columns the quantisers index with 32 bits
+constexpr int kMaxGemmDim = 1 << 16;
+
+bool dtype_ok(int d) { return d == SAMPLER_DTYPE_F32 || d == SAMPLER_DTYPE_BF16 || d == SAMPLER_DTYPE_F16; }
+size_t dtype_size(int d) { return d == SAMPLER_DTYPE_F32 ? 4 : 2; }
+size_t pad256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+int check_filter_args(const SamplerFilterConfig* cfg, int batch, const float* temperature_rows, const float* coins,
+                      const unsigned long long* rng_state, const int* out_ids) {
+    if (!cfg || !out_ids) return fail(SAMPLER_E_INVALID, "null config or out_ids");
+    if (batch < 0 || cfg->vocab_size < 1)
+        return fail(SAMPLER_E_INVALID, "bad sizes: batch=%d vocab=%d", batch, cfg->vocab_size);
+    if (cfg->vocab_size > SAMPLER_FILTERED_MAX_VOCAB)
+        return fail(SAMPLER_E_UNSUPPORTED, "vocab_size %d above SAMPLER_FILTERED_MAX_VOCAB %d", cfg->vocab_size,
+                    SAMPLER_FILTERED_MAX_VOCAB);
+    if (!dtype_ok(cfg->logits_dtype)) return fail(SAMPLER_E_INVALID, "unknown logits_dtype %d", cfg->logits_dtype);
+    const bool all_greedy = !temperature_rows && !(cfg->temperature >= 1e-6f);
+    if (!all_greedy && !coins && !rng_state)
+        return fail(SAMPLER_E_INVALID, "coins and rng_state are NULL but rows need a coin");
+    return SAMPLER_OK;
+}
+
+int quantize_call(const void* x, int x_dtype, const float* norm_weight, int rows, int dim, long long ld,
+                  int block_rows, void* out_q, float* out_scales, cudaStream_t stream) {
+    g_last_launches = 0;
+    if (!x || !out_q || !out_scales) return fail(SAMPLER_E_INVALID, "null x, out_q or out_scales");
+    if (!dtype_ok(x_dtype)) return fail(SAMPLER_E_INVALID, "unknown x_dtype %d", x_dtype);
+    if (rows < 0 || dim < 1 || ld < dim)
+        return fail(SAMPLER_E_INVALID, "bad sizes: rows=%d dim=%d ld=%lld", rows, dim, ld);
+    if (dim > kMaxDim) return fail(SAMPLER_E_UNSUPPORTED, "dim %d above %d", dim, kMaxDim);
+    if (block_rows != 1 && block_rows != 128) return fail(SAMPLER_E_INVALID, "block_rows %d is not 1 or 128", block_rows);
+    const size_t size = dtype_size(x_dtype);
+    if (((uintptr_t)x & (size - 1)) || ((uintptr_t)out_scales & 3u) || ((uintptr_t)norm_weight & 3u))
+        return fail(SAMPLER_E_INVALID, "x, norm_weight or out_scales not aligned to its elements");
+    const long long blocks = (((long long)rows + 127) / 128) * ((dim + 127) / 128);
+    if (block_rows == 128 && blocks > 0x7FFFFFFFLL)
+        return fail(SAMPLER_E_UNSUPPORTED, "%lld blocks in one call", blocks);
+    if (rows == 0) return SAMPLER_OK;
+    DeviceCtx* c = nullptr;
+    const int rc = get_ctx(&c);
+    if (rc) return rc;
+    b2s::QuantLaunch q{};
+    q.x = x;
+    q.dtype = x_dtype;
+    q.ld = ld;
+    q.rows = rows;
+    q.dim = dim;
+    q.block_rows = block_rows;
+    q.norm_weight = norm_weight;
+    q.q = out_q;
+    q.scales = out_scales;
+    const int n = b2s::launch_quantize_fp8(q, c->num_sms, stream);
+    if (n < 0) return fail(SAMPLER_E_CUDA, "quantize launch: %s", cudaGetErrorString((cudaError_t)(-n)));
+    g_last_launches = n;
+    return SAMPLER_OK;
+}
+}  // namespace
+
+extern "C" {
+
+int sampler_filtered(const SamplerFilterConfig* cfg, const void* logits, int batch, long long ld,
+                     const float* temperature_rows, const int* topk_rows, const float* topp_rows,
+                     const float* minp_rows, const float* coins, unsigned long long* rng_state, int* out_ids,
+                     float* out_logprobs, int* out_kept, int* row_flags, void* stream) {
+    g_last_launches = 0;
+    int rc = check_filter_args(cfg, batch, temperature_rows, coins, rng_state, out_ids);
+    if (rc) return rc;
+    if (!logits || ld < cfg->vocab_size)
+        return fail(SAMPLER_E_INVALID, "null logits, or ld %lld below vocab %d", ld, cfg->vocab_size);
+    if ((uintptr_t)logits & (dtype_size(cfg->logits_dtype) - 1))
+        return fail(SAMPLER_E_INVALID, "logits not aligned to its elements");
+    if (batch == 0) return SAMPLER_OK;
+    DeviceCtx* c = nullptr;
+    rc = get_ctx(&c);
+    if (rc) return rc;
+    b2s::FilterLaunch f{};
+    f.logits = logits;
+    f.dtype = cfg->logits_dtype;
+    f.ld = ld;
+    f.batch = batch;
+    f.vocab = cfg->vocab_size;
+    f.temperature = cfg->temperature;
+    f.topk = cfg->topk;
+    f.topp = cfg->topp;
+    f.minp = cfg->minp;
+    f.temperature_rows = temperature_rows;
+    f.topk_rows = topk_rows;
+    f.topp_rows = topp_rows;
+    f.minp_rows = minp_rows;
+    f.coins = coins;
+    f.rng_state = rng_state;
+    f.out_ids = out_ids;
+    f.logprobs = out_logprobs;
+    f.kept = out_kept;
+    f.row_flags = row_flags;
+    const int n = b2s::launch_filtered_sample(f, c->num_sms, (cudaStream_t)stream);
+    if (n < 0) return fail(SAMPLER_E_CUDA, "filtered sampler launch: %s", cudaGetErrorString((cudaError_t)(-n)));
+    g_last_launches = n;
+    return SAMPLER_OK;
+}
+
+int quantize_fp8(const void* x, int x_dtype, int rows, int dim, long long ld, int block_rows, void* out_q,
+                 float* out_scales, void* stream) {
+    return quantize_call(x, x_dtype, nullptr, rows, dim, ld, block_rows, out_q, out_scales, (cudaStream_t)stream);
+}
+
+int rmsnorm_fp8(const void* x, int x_dtype, const float* norm_weight, int batch, int dim, long long ld, void* out_q,
+                float* out_scales, void* stream) {
+    if (!norm_weight) return fail(SAMPLER_E_INVALID, "null norm_weight");
+    return quantize_call(x, x_dtype, norm_weight, batch, dim, ld, 1, out_q, out_scales, (cudaStream_t)stream);
+}
+
+int classifier_logits_fp8(const void* hidden, const float* hidden_scales, const void* wcls, const float* wcls_scales,
+                          int batch, int dim, int vocab, void* logits_out, int logits_dtype, long long ld,
+                          void* stream) {
+    g_last_launches = 0;
+    if (!hidden || !hidden_scales || !wcls || !wcls_scales || !logits_out)
+        return fail(SAMPLER_E_INVALID, "null hidden, wcls, scales or logits_out");
+    if (logits_dtype != SAMPLER_DTYPE_F32 && logits_dtype != SAMPLER_DTYPE_BF16)
+        return fail(SAMPLER_E_INVALID, "logits_dtype %d is not F32 or BF16", logits_dtype);
+    if (batch < 0 || dim < 16 || (dim % 16) != 0 || vocab < 1 || ld < vocab)
+        return fail(SAMPLER_E_INVALID, "bad sizes: batch=%d dim=%d (multiple of 16) vocab=%d ld=%lld", batch, dim,
+                    vocab, ld);
+    if (dim > kMaxGemmDim) return fail(SAMPLER_E_UNSUPPORTED, "dim %d above %d", dim, kMaxGemmDim);
+    if (((uintptr_t)hidden & 15u) || ((uintptr_t)wcls & 15u))
+        return fail(SAMPLER_E_INVALID, "hidden and wcls must be 16-byte aligned");
+    if (((uintptr_t)hidden_scales & 3u) || ((uintptr_t)wcls_scales & 3u) ||
+        ((uintptr_t)logits_out & (dtype_size(logits_dtype) - 1)))
+        return fail(SAMPLER_E_INVALID, "scales or logits_out not aligned to its elements");
+    if (((long long)batch + 127) / 128 * (((long long)vocab + 15) / 16) > 0x3FFFFFFFLL)
+        return fail(SAMPLER_E_UNSUPPORTED, "batch %d by vocab %d is too large for one call", batch, vocab);
+    if (batch == 0) return SAMPLER_OK;
+    DeviceCtx* c = nullptr;
+    const int rc = get_ctx(&c);
+    if (rc) return rc;
+    b2s::Fp8GemmLaunch g{};
+    g.h = hidden;
+    g.h_scales = hidden_scales;
+    g.w = wcls;
+    g.w_scales = wcls_scales;
+    g.batch = batch;
+    g.dim = dim;
+    g.vocab = vocab;
+    g.logits = logits_out;
+    g.out_bf16 = logits_dtype == SAMPLER_DTYPE_BF16 ? 1 : 0;
+    g.ld = ld;
+    g.error_word = c->error_word;
+    const int n = b2s::launch_fp8_gemm(g, c->num_sms, (cudaStream_t)stream);
+    if (n < 0) return fail(SAMPLER_E_CUDA, "8-bit classifier launch: %s", cudaGetErrorString((cudaError_t)(-n)));
+    g_last_launches = n;
+    return SAMPLER_OK;
+}
+
+size_t classifier_fp8_workspace_bytes(int batch, int dim, int vocab, int logits_dtype) {
+    if (batch < 1 || dim < 1 || vocab < 1) return 0;
+    const size_t blocks = ((size_t)dim + 127) / 128;
+    const size_t operand = pad256((size_t)batch * dim) + pad256((size_t)batch * blocks * sizeof(float));
+    return operand + (logits_dtype < 0 ? 0 : (size_t)batch * vocab * dtype_size(logits_dtype));
+}
+
+int classifier_fp8_sample_filtered(const SamplerFilterConfig* cfg, const void* x, int x_dtype,
+                                   const float* norm_weight, const void* wcls, const float* wcls_scales, int batch,
+                                   int dim, const float* temperature_rows, const int* topk_rows,
+                                   const float* topp_rows, const float* minp_rows, const float* coins,
+                                   unsigned long long* rng_state, int* out_ids, float* out_logprobs, int* out_kept,
+                                   void* logits_out, int* row_flags, void* workspace, size_t workspace_bytes,
+                                   void* stream) {
+    g_last_launches = 0;
+    int rc = check_filter_args(cfg, batch, temperature_rows, coins, rng_state, out_ids);
+    if (rc) return rc;
+    // checked here, before the first of the launches, so that a refused call writes nothing
+    if (!x || !wcls || !wcls_scales) return fail(SAMPLER_E_INVALID, "null x, wcls or wcls_scales");
+    if (!dtype_ok(x_dtype)) return fail(SAMPLER_E_INVALID, "unknown x_dtype %d", x_dtype);
+    if (cfg->logits_dtype == SAMPLER_DTYPE_F16)
+        return fail(SAMPLER_E_INVALID, "logits_dtype of the classifier is F32 or BF16");
+    if (dim < 16 || (dim % 16) != 0) return fail(SAMPLER_E_INVALID, "dim %d is not a multiple of 16", dim);
+    if (dim > kMaxGemmDim) return fail(SAMPLER_E_UNSUPPORTED, "dim %d above %d", dim, kMaxGemmDim);
+    const size_t lsize = dtype_size(cfg->logits_dtype);
+    if (((uintptr_t)wcls & 15u) || ((uintptr_t)wcls_scales & 3u) || ((uintptr_t)logits_out & (lsize - 1)))
+        return fail(SAMPLER_E_INVALID, "wcls not 16-byte aligned, or wcls_scales or logits_out not to its elements");
+    if (batch == 0) return SAMPLER_OK;
+    const int V = cfg->vocab_size;
+    const size_t need = classifier_fp8_workspace_bytes(batch, dim, V, logits_out ? -1 : cfg->logits_dtype);
+    if (!workspace || workspace_bytes < need)
+        return fail(SAMPLER_E_WORKSPACE, "workspace %zu bytes < required %zu", workspace ? workspace_bytes : (size_t)0,
+                    need);
+    if ((uintptr_t)workspace & 15u) return fail(SAMPLER_E_INVALID, "workspace not 16-byte aligned");
+    char* hq = static_cast<char*>(workspace);
+    float* hs = reinterpret_cast<float*>(hq + pad256((size_t)batch * dim));
+    void* logits = logits_out ? logits_out : hq + classifier_fp8_workspace_bytes(batch, dim, V, -1);
+    rc = quantize_call(x, x_dtype, norm_weight, batch, dim, dim, 1, hq, hs, (cudaStream_t)stream);
+    if (rc) return rc;
+    int launches = g_last_launches;
+    rc = classifier_logits_fp8(hq, hs, wcls, wcls_scales, batch, dim, V, logits, cfg->logits_dtype, V, stream);
+    if (rc) return rc;
+    launches += g_last_launches;
+    rc = sampler_filtered(cfg, logits, batch, V, temperature_rows, topk_rows, topp_rows, minp_rows, coins, rng_state,
+                          out_ids, out_logprobs, out_kept, row_flags, stream);
+    g_last_launches += launches;
+    return rc;
 }
 
 int sampler_batched_host(const SamplerBatchConfig* cfg, const float* logits, int batch, long long ld,

@@ -322,8 +322,8 @@ typedef struct {
  *                    with T >= 1e-6 (neither read nor written with coins)
  *   out_ids          [batch] token ids; 0 on a row without candidates, which is
  *                    flagged SAMPLER_ROW_NO_CANDIDATE
- *   out_logprobs     [batch] or NULL: ln(w_id / mass of the n); -infinity
- *                    without candidates
+ *   out_logprobs     [batch] or NULL: ln(w_id / mass of the n), the mass within
+ *                    2^-17 relative; -infinity without candidates
  *   out_kept         [batch] or NULL: n
  *   row_flags        [batch] or NULL: SAMPLER_ROW_NAN, SAMPLER_ROW_NO_CANDIDATE
  * Weights and sums that decide an id are held to about 2^-43 of the largest

@@ -34,6 +34,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 namespace b2s {
 namespace {
 
@@ -303,79 +305,115 @@ __device__ __noinline__ void sample_exact(const FilterLaunch& p, int r, RowRule 
 constexpr int kListCap = 1024;     // entries that can be sorted on chip
 constexpr int kBinCap = 2048;      // bins of a histogram
 constexpr int kChunkBins = 512;    // bins of the chunk maxima
-constexpr int kChunkCap = 2048;    // chunk maxima kept
-constexpr int kInFlight = 4;       // vectors a lane loads before it uses them
-constexpr float kLog2e = 1.4426950408889634f;
-
-struct Bracket {
-    float lo, hi;        // bin coordinates [lo, hi) of the bins that hold the crossing; "above" is below lo
-    double mass;         // of the entries above
-    int above;           // their number
-    int n;               // entries in the bracket's list
-};
+constexpr int kChunkCap = 2048;    // chunk maxima kept: 64 groups of batches, one a lane
+constexpr int kU = 4;              // vectors of a lane in a batch
+constexpr int kWarpList = 64;      // a list of up to this many is one warp's work
+constexpr float kLowest = -3.402823466e38f;
 
 template <int NT>
 struct FastSmem {
     union {
         struct {
-            unsigned mass[kBinCap];
-            unsigned count[kBinCap];
+            unsigned bin[kBinCap];
         } hist;
+        unsigned chunk_bin[kChunkBins];  // zero when pass 2 starts, over before the list does
         struct {
             u64 key[kListCap];   // sorted: falling value, rising index
-            double cum[kListCap];
+            union {
+                double cum[kListCap];
+                int hit[kChunkCap];  // chunks that hold entries above the threshold
+            };
         } list;
         ExactSmem exact;
     };
-    float chunk_max[kChunkCap + 4];  // a row that starts between two boundaries has one strip more
+    float chunk_max[kChunkCap];
     double red_d[NT / 32];
-    float red_f[4][NT / 32];
-    unsigned red_u[2][NT / 32];
+    float red_f[4][NT / 32];  // by warp: maximum, minimum, smallest chunk maximum, reference of the sum
+    unsigned red_u[NT / 32];
     float coin;
     unsigned n[2];
+    unsigned hits;
     int bin[4];
-    unsigned cut_count;
     int status;
     int first;
 };
 
 // A row as 16-byte vectors from the 16-byte boundary at or before its first
 // element: `lead` elements of vector 0 and the end of the last one are not the
-// row's and are neither read nor seen (they count as -infinity).
+// row's and are neither read nor seen (they count as -infinity).  A warp loads
+// batches of 32 * kU vectors, of which lane l has vectors l, l + 32, ..
 template <typename T>
 struct VecRow {
     static constexpr int E = 16 / sizeof(T);
     const T* base;
-    int lead, vocab, vecs;
+    int lead, vocab, vecs, batches;
+    int whole_from;
+    unsigned whole_count;
     __device__ __forceinline__ VecRow(const T* x, int v) {
         lead = (int)((reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(T));
         base = x - lead;
         vocab = v;
         vecs = (lead + v + E - 1) / E;
+        batches = (vecs + 32 * kU - 1) / (32 * kU);
+        whole_from = lead ? 1 : 0;
+        whole_count = (unsigned)max((lead + v) / E - whole_from, 0);
     }
     __device__ __forceinline__ int index(int vec, int e) const { return vec * E + e - lead; }
-    __device__ __forceinline__ bool whole(int vec) const { return vec * E >= lead && (vec + 1) * E <= lead + vocab; }
-    __device__ __forceinline__ void load(int vec, float (&v)[E]) const {
-        if (whole(vec)) {
-            const uint4 u = __ldg(reinterpret_cast<const uint4*>(base) + vec);
-            unpack(u, v);
-        } else {
+    __device__ __forceinline__ bool whole(int vec) const { return (unsigned)(vec - whole_from) < whole_count; }
+    __device__ __forceinline__ uint4 load(int vec) const {
+        if (whole(vec)) return __ldg(reinterpret_cast<const uint4*>(base) + vec);
+        constexpr uint32_t none = sizeof(T) == 4 ? 0xFF800000u : std::is_same<T, __half>::value ? 0xFC00FC00u : 0xFF80FF80u;
+        uint4 u = make_uint4(none, none, none, none);
+        if (vec < vecs) {
+            uint32_t w[4] = {none, none, none, none};
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 const int i = index(vec, e);
-                v[e] = (i >= 0 && i < vocab) ? as_f32<T>(base[lead + i]) : -__int_as_float(0x7F800000);
+                if (i >= 0 && i < vocab) {
+                    if (sizeof(T) == 4) {
+                        w[e & 3] = reinterpret_cast<const uint32_t*>(base)[lead + i];
+                    } else {
+                        const uint32_t h = reinterpret_cast<const unsigned short*>(base)[lead + i];
+                        const int s = 16 * (e & 1);
+                        w[(e >> 1) & 3] = (w[(e >> 1) & 3] & ~(0xFFFFu << s)) | (h << s);
+                    }
+                }
+            }
+            u = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        return u;
+    }
+    __device__ __forceinline__ void load_batch(int batch, int lane, uint4 (&raw)[kU]) const {
+        const int first = batch * 32 * kU;
+        if (first >= whole_from && first + 32 * kU <= whole_from + (int)whole_count) {
+            const uint4* q = reinterpret_cast<const uint4*>(base) + first + lane;
+#pragma unroll
+            for (int u = 0; u < kU; ++u) raw[u] = __ldg(q + 32 * u);
+        } else {
+#pragma unroll 1
+            for (int u = 0; u < kU; ++u) {
+                const uint4 w = load(first + 32 * u + lane);
+                if (u == 0) raw[0] = w;
+                if (u == 1) raw[1] = w;
+                if (u == 2) raw[2] = w;
+                if (u == 3) raw[3] = w;
             }
         }
     }
-    __device__ __forceinline__ static void unpack(const uint4& u, float (&v)[E]) {
+    __device__ __forceinline__ static void widen(const uint4& u, float (&v)[E]) {
         const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(w[i]);
-        } else {
-            const T* t = reinterpret_cast<const T*>(&u);
-#pragma unroll
-            for (int i = 0; i < E; ++i) v[i] = as_f32<T>(t[i]);
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 4) {
+                v[i] = __uint_as_float(w[i]);
+            } else if constexpr (std::is_same<T, __half>::value) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+                v[2 * i] = f.x;
+                v[2 * i + 1] = f.y;
+            } else {
+                v[2 * i] = __uint_as_float(w[i] << 16);
+                v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+            }
         }
     }
 };
@@ -385,13 +423,56 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
-__device__ __forceinline__ float warp_max_nan(float v) {
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// Largest of a vector's elements, NaN if one is.
+template <int E>
+__device__ __forceinline__ float vec_max(const float (&v)[E]) {
+    float m = max_nan(v[0], v[1], v[2]);
 #pragma unroll
-    for (int o = 16; o; o >>= 1) v = max_nan(v, __shfl_xor_sync(kFullMask, v, o));
-    return v;
+    for (int e = 3; e + 1 < E; e += 2) m = max_nan(m, v[e], v[e + 1]);
+    return max_nan(m, v[E - 1]);
+}
+__device__ __forceinline__ float warp_max(float v) {
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ float warp_max_nan(float v) {
+    float r;
+    asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ float warp_min(float v) {
+    float r;
+    asm volatile("redux.sync.min.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
 }
 
-// Sum of `n` values as a tree.
+// Two fp32 numbers in one register pair, and the instructions on them.
+__device__ __forceinline__ u64 pack2(float a, float b) {
+    u64 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpack2(u64 v, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ u64 fma2(u64 a, u64 b, u64 c) {
+    u64 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ u64 add2(u64 a, u64 b) {
+    u64 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+// Sum of N values as a tree.
 template <int N>
 __device__ __forceinline__ float tree_sum(float (&t)[N]) {
 #pragma unroll
@@ -399,6 +480,27 @@ __device__ __forceinline__ float tree_sum(float (&t)[N]) {
 #pragma unroll
         for (int i = 0; i < h; ++i) t[i] += t[i + h];
     return t[0];
+}
+
+// 2^t for t up to 1 (0 below -1000), 2^-44 relative: n = rint(t), and
+// 1 + f * P(f) for 2^f, f = t - n, P of degree 8 interpolating (2^f - 1) / f at
+// the Chebyshev nodes of [-1/2, 1/2].
+__device__ __forceinline__ double exp2_64(double t) {
+    const double big = 6755399441055744.0;  // 1.5 * 2^52: its sum with t holds rint(t) in the low word
+    const double s = t + big;
+    const double f = t - (s - big);
+    double p = 0x1.b63880a30e9ffp-24;
+    p = fma(p, f, 0x1.63d136366db24p-20);
+    p = fma(p, f, 0x1.ffcb9515a8016p-17);
+    p = fma(p, f, 0x1.4308ac85aa947p-13);
+    p = fma(p, f, 0x1.5d87fe86fe88ep-10);
+    p = fma(p, f, 0x1.3b2ab7181b755p-7);
+    p = fma(p, f, 0x1.c6b08d7047e52p-5);
+    p = fma(p, f, 0x1.ebfbdff823cedp-3);
+    p = fma(p, f, 0x1.62e42fefa39efp-1);
+    p = fma(p, f, 1.0);
+    const double r = __hiloint2double(__double2hiint(p) + (__double2loint(s) << 20), __double2loint(p));
+    return t >= -1000.0 ? r : 0.0;
 }
 
 // Inclusive scan over the CTA's threads.  `part` holds one entry a warp.
@@ -413,18 +515,19 @@ __device__ __forceinline__ V block_scan(V v, V* part) {
     if (lane == 31) part[warp] = v;
     __syncthreads();
     V before = 0;
-    for (int w = 0; w < warp; ++w) before += part[w];
+#pragma unroll
+    for (int w = 0; w < NT / 32; ++w) before += w < warp ? part[w] : V(0);
     __syncthreads();
     return v + before;
 }
-template <int NT>
-__device__ __forceinline__ double block_sum(double v, double* part) {
+template <int NT, typename V>
+__device__ __forceinline__ V block_sum(V v, V* part) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(kFullMask, v, o);
     if (lane == 0) part[warp] = v;
     __syncthreads();
-    double t = 0.0;
+    V t = 0;
 #pragma unroll
     for (int w = 0; w < NT / 32; ++w) t += part[w];
     __syncthreads();
@@ -435,128 +538,143 @@ __device__ __forceinline__ double block_sum(double v, double* part) {
 struct RowFacts {
     float top;         // the largest logit
     float low_chunk;   // the smallest finite chunk maximum
-    float z;           // log2(e) / T
-    double sum;        // mass of the row, off by up to sum_err of it
-    double sum_err;
-    float low;         // the smallest logit; -infinity when some are masked by it
+    float z;           // log2(e) / T, as one fp32 number
+    double z64;
+    float sum;         // mass of the row (the top's is 1), off by up to sum_err of it
+    float sum_err;
+    float low;         // the smallest logit where pass 1 was asked for it, else -infinity
     float minp_at;     // logits of at least this pass min-p (-infinity when off)
     int chunks;
-    int chunk_shift;   // log2 of the 32-vector strips of a chunk
+    int chunk_shift;   // log2 of the batches of a chunk
+    __device__ __forceinline__ double weight(float x) const { return exp2_64(((double)x - (double)top) * z64); }
 };
-
-// Bound of |sum - true mass| / mass for fp32 weights 2^((x - top) * z), in
-// units of 2^-24: the roundings of the difference, of z and of the product make
-// 3 ln 2 |log2 w| of a weight, ex2 4; the mean of |log2 w| under the weights is
-// H - log2 S <= log2(V / S) bits; the trees have 5 levels, and each change of a
-// running maximum costs another ex2 and its argument's error (|d| 2^-d < 0.54
-// of the older part).  Sums of trees are fp64.
-__device__ __forceinline__ double sum_error(float sum, int vocab, int rescalings) {
-    const float bits = fmaxf(__log2f((float)vocab / sum), 0.0f) + 1.0f;
-    return 5.97e-8 * (2.1 * (double)bits + 10.0 + 6.0 * (rescalings + 1));
-}
 
 enum { kDone = 0, kNeedSum64 = 1, kNeedBins = 2, kNeedExact = 3 };
 
-// Pass 1.  False when the row is for sample_exact (NaN, infinite or no maximum).
-template <int NT, typename T>
-__device__ bool first_pass(const VecRow<T>& row, FastSmem<NT>& sm, RowFacts& f) {
+// Pass 1: maximum, chunk maxima and mass; with kLow the minimum too (an open
+// row with -infinity among its entries has to count its candidates).  A chunk is
+// what one lane reads of 2^chunk_shift batches.  Weights are 2^(x * z - R) with
+// an integer R, z in two words: two FMAs with one rounding each, and a new R (when
+// a weight would pass 2^60) rescales by a power of two, exactly.  So a weight is
+// off by 2 * 2^-25 * ln 2 * |log2 w| relative and ex2's 2^-22, the trees by 5
+// steps; the mean of |log2 w| under the weights is H - log2 S <= log2(V / S) bits.
+// Sums of trees are fp64.
+template <int NT, typename T, bool kLow>
+__device__ __forceinline__ void first_pass(const VecRow<T>& row, int shift, uint4 (&next)[kU], FastSmem<NT>& sm,
+                                           RowFacts& f) {
     constexpr int E = VecRow<T>::E;
+    constexpr int NW = NT / 32;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const float inf = __int_as_float(0x7F800000);
-    const int strips = (row.vecs + 31) >> 5;
-    f.chunk_shift = strips > kChunkCap ? 2 : 0;
-    f.chunks = (strips + (1 << f.chunk_shift) - 1) >> f.chunk_shift;
-    float run_max = -3.402823466e38f, top = -inf, low = inf, low_chunk = inf;
+    const float z_hi = __double2float_rd(f.z64);
+    const float z_lo = fmaxf(__double2float_rd(f.z64 - (double)z_hi), 1e-37f);  // above 0: -infinity stays itself
+    const int group = (1 << shift) - 1;
+    const u64 zz_hi = pack2(z_hi, z_hi), zz_lo = pack2(z_lo, z_lo);
+    float ref = 0.0f, limit = -inf, top = -inf, chunk = -inf, low = inf, low_chunk = inf;
     double run_sum = 0.0;
-    int rescalings = 0;
-    for (int s0 = warp * kInFlight; s0 < strips; s0 += (NT / 32) * kInFlight) {
-        float v[kInFlight][E];
+    int b = warp << shift;
+    while (b < row.batches) {
+        uint4 raw[kU];
 #pragma unroll
-        for (int u = 0; u < kInFlight; ++u) row.load((s0 + u) * 32 + lane, v[u]);
-        float group = -inf;
+        for (int u = 0; u < kU; ++u) raw[u] = next[u];
+        const int now = b;
+        b = ((b + 1) & group) ? b + 1 : b + 1 + ((NW - 1) << shift);
+        if (b < row.batches) row.load_batch(b, lane, next);  // on its way while this one is used
+        float m = -inf;
 #pragma unroll
-        for (int u = 0; u < kInFlight; ++u) {
-            const int vec = (s0 + u) * 32 + lane;
-            float m = v[u][0], l = v[u][0];
+        for (int u = 0; u < kU; ++u) {
+            float v[E];
+            VecRow<T>::widen(raw[u], v);
 #pragma unroll
-            for (int e = 1; e < E; ++e) {
-                m = max_nan(m, v[u][e]);
-                l = fminf(l, v[u][e]);
-            }
-            if (row.whole(vec)) {
-                low = fminf(low, l);
-            } else {
+            for (int e = 0; e < E; e += 2) m = max_nan(m, v[e], v[e + 1]);
+            if (kLow) {
+                const int vec = (now * kU + u) * 32 + lane;
 #pragma unroll
                 for (int e = 0; e < E; ++e)
-                    if (row.index(vec, e) >= 0 && row.index(vec, e) < row.vocab) low = fminf(low, v[u][e]);
+                    if (row.whole(vec) || (row.index(vec, e) >= 0 && row.index(vec, e) < row.vocab)) low = fminf(low, v[e]);
             }
-            m = warp_max_nan(m);
-            if (f.chunk_shift == 0) {
-                if (lane == 0 && s0 + u < strips) sm.chunk_max[s0 + u] = m;
-                if (m > -inf) low_chunk = fminf(low_chunk, m);
+        }
+        chunk = max_nan(chunk, m);
+        if (b >= row.batches || (b >> shift) != (now >> shift)) {
+            sm.chunk_max[((now >> shift) << 5) | lane] = chunk;
+            low_chunk = fminf(low_chunk, chunk > -inf ? chunk : inf);
+            top = max_nan(top, chunk);
+            chunk = -inf;
+        }
+        if (__any_sync(kFullMask, m > limit)) {
+            const float r = rintf(warp_max(m) * z_hi), d = ref - r;
+            run_sum *= limit > -inf && d > -126.0f ? (double)__int_as_float((127 + (int)d) << 23) : 0.0;
+            ref = r;
+            limit = (r + 60.0f) / z_hi;
+        }
+        const u64 rr = pack2(-ref, -ref);
+        u64 t[kU];
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+            float v[E];
+            VecRow<T>::widen(raw[u], v);
+            u64 w[E / 2];
+#pragma unroll
+            for (int i = 0; i < E / 2; ++i) {
+                const u64 x = pack2(v[2 * i], v[2 * i + 1]);
+                float a, c;
+                unpack2(fma2(x, zz_lo, fma2(x, zz_hi, rr)), a, c);
+                w[i] = pack2(ex2_approx(a), ex2_approx(c));
             }
-            group = max_nan(group, m);
-        }
-        if (f.chunk_shift != 0) {
-            if (lane == 0) sm.chunk_max[s0 >> 2] = group;
-            if (group > -inf) low_chunk = fminf(low_chunk, group);
-        }
-        top = max_nan(top, group);
-        if (group > run_max) {  // the whole warp's
-            run_sum *= (double)ex2_approx((run_max - group) * f.z);
-            run_max = group;
-            ++rescalings;
-        }
-        float t[kInFlight];
 #pragma unroll
-        for (int u = 0; u < kInFlight; ++u) {
+            for (int h = E / 4; h; h /= 2)
 #pragma unroll
-            for (int e = 0; e < E; ++e) v[u][e] = ex2_approx((v[u][e] - run_max) * f.z);
-            t[u] = tree_sum(v[u]);
+                for (int i = 0; i < h; ++i) w[i] = add2(w[i], w[i + h]);
+            t[u] = w[0];
         }
-        run_sum += (double)tree_sum(t);
+        float a, c;
+        unpack2(add2(add2(t[0], t[1]), add2(t[2], t[3])), a, c);
+        run_sum += (double)(a + c);
     }
-    // the maxima are a warp's; the sums and the minimum a lane's
+    // all of these are a lane's; then a warp's; then the row's, in every warp
+    top = warp_max_nan(top);
+    low_chunk = warp_min(low_chunk);
+    if (kLow) low = warp_min(low);
 #pragma unroll
-    for (int o = 16; o; o >>= 1) low = fminf(low, __shfl_xor_sync(kFullMask, low, o));
+    for (int o = 16; o; o >>= 1) run_sum += __shfl_xor_sync(kFullMask, run_sum, o);
     if (lane == 0) {
         sm.red_f[0][warp] = top;
         sm.red_f[1][warp] = low;
         sm.red_f[2][warp] = low_chunk;
-        sm.red_u[0][warp] = (unsigned)rescalings;
+        sm.red_f[3][warp] = ref;
+        sm.red_d[warp] = run_sum;
     }
     __syncthreads();
-    top = -inf;
-    low = low_chunk = inf;
+    const int w = lane < NW ? lane : 0;
+    top = warp_max_nan(sm.red_f[0][w]);
+    if (kLow) low = warp_min(sm.red_f[1][w]);
+    low_chunk = warp_min(sm.red_f[2][w]);
+    const float all = rintf(top * z_hi);
+    double s = lane < NW ? sm.red_d[w] * exp2_64(fmin((double)(sm.red_f[3][w] - all), 0.0)) : 0.0;
 #pragma unroll
-    for (int w = 0; w < NT / 32; ++w) {
-        top = max_nan(top, sm.red_f[0][w]);
-        low = fminf(low, sm.red_f[1][w]);
-        low_chunk = fminf(low_chunk, sm.red_f[2][w]);
-        rescalings = max(rescalings, (int)sm.red_u[0][w]);
-    }
-    f.sum = block_sum<NT>(run_sum * (double)ex2_approx((run_max - top) * f.z), sm.red_d);
-    f.sum_err = sum_error((float)f.sum, row.vocab, rescalings + 1);
+    for (int o = NW / 2; o; o >>= 1) s += __shfl_xor_sync(kFullMask, s, o);
+    s = __shfl_sync(kFullMask, s, 0);
+    f.sum = (float)(s * exp2_64((double)all - (double)top * f.z64));
+    const float bits = fmaxf(__log2f((float)row.vocab / f.sum), 0.0f) + 1.0f;
+    f.sum_err = 6e-8f * (0.7f * bits + 11.0f);  // units of 2^-24; the sum's own rounding and half a bit of R among them
     f.top = top;
-    f.low = low;
+    f.low = kLow ? low : -inf;
     f.low_chunk = low_chunk;
-    return top > -inf && top < inf;
+    f.chunk_shift = shift;
+    f.chunks = ((row.batches + group) >> shift) << 5;
 }
 
-// The mass in fp64 of the entries whose key is at least `limit`, and their number.
+// The mass in fp64 of the whole row.
 template <int NT, typename T>
-__device__ __noinline__ double sum64(const VecRow<T>& row, float top, double temperature, u64 limit, FastSmem<NT>& sm) {
+__device__ __noinline__ double sum64(const VecRow<T>& row, const RowFacts& f, FastSmem<NT>& sm) {
     constexpr int E = VecRow<T>::E;
+    const double c = -(double)f.top * f.z64;
     double s = 0.0;
-    for (int v0 = threadIdx.x; v0 < row.vecs; v0 += NT) {
+    for (int vec = threadIdx.x; vec < row.vecs; vec += NT) {
         float v[E];
-        row.load(v0, v);
+        VecRow<T>::widen(row.load(vec), v);
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const uint32_t k = order_key(v[e]);
-            if (k != 0u && (((u64)k << 32) | (0xFFFFFFFFu - (uint32_t)row.index(v0, e))) >= limit)
-                s += weight64(v[e], top, temperature);
-        }
+        for (int e = 0; e < E; ++e) s += exp2_64(fma((double)v[e], f.z64, c));
     }
     return block_sum<NT>(s, sm.red_d);
 }
@@ -564,14 +682,14 @@ __device__ __noinline__ double sum64(const VecRow<T>& row, float top, double tem
 template <int NT, typename T>
 __device__ __noinline__ int count_candidates(const VecRow<T>& row, FastSmem<NT>& sm) {
     constexpr int E = VecRow<T>::E;
-    int c = 0;
-    for (int v0 = threadIdx.x; v0 < row.vecs; v0 += NT) {
+    unsigned c = 0;
+    for (int vec = threadIdx.x; vec < row.vecs; vec += NT) {
         float v[E];
-        row.load(v0, v);
+        VecRow<T>::widen(row.load(vec), v);
 #pragma unroll
         for (int e = 0; e < E; ++e) c += v[e] > -__int_as_float(0x7F800000);
     }
-    return (int)block_sum<NT>((double)c, sm.red_d);
+    return (int)block_sum<NT>(c, sm.red_u);
 }
 
 // Appends the entries of one vector that `mask` selects to a list of (key, index).
@@ -588,34 +706,78 @@ __device__ __forceinline__ void push_entries(const VecRow<T>& row, int vec, cons
         }
 }
 
-// Sorts list[0 .. n) of at most kListCap keys, falling.
+// One compare-exchange step of a bitonic network over 128 keys of a warp
+// (key r * 32 + lane), `first` the index of key 0 in the whole array.
+__device__ __forceinline__ void warp_step(u64 (&k)[4], int first, int size, int stride, int lane) {
+    u64 o[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+        o[r] = stride == 64 ? k[r ^ 2] : stride == 32 ? k[r ^ 1] : __shfl_xor_sync(kFullMask, k[r], stride);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int i = first + r * 32 + lane;
+        const bool take_max = ((i & stride) == 0) == ((i & size) == 0);
+        k[r] = take_max ? (k[r] > o[r] ? k[r] : o[r]) : (k[r] < o[r] ? k[r] : o[r]);
+    }
+}
+
+// Sorts list[0 .. n) of at most kListCap keys, falling: bitonic, in which the
+// steps inside 128 keys are a warp's own and only those across pass through
+// shared memory and a barrier (9 for 1024 keys, not 55).
 template <int NT>
 __device__ void sort_list(u64* list, int n) {
-    if (n <= 64) {
-        if (threadIdx.x < 32) warp_sort_desc<2>(list, n, threadIdx.x & 31);
-        __syncthreads();
-        return;
-    }
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int P = 128;
     while (P < n) P <<= 1;
-    for (int i = n + threadIdx.x; i < P; i += NT) list[i] = 0ull;
+    for (int first = warp * 128; first < P; first += NT / 32 * 128) {
+        u64 k[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) k[r] = first + r * 32 + lane < n ? list[first + r * 32 + lane] : 0ull;
+#pragma unroll
+        for (int size = 2; size <= 128; size <<= 1)
+#pragma unroll
+            for (int stride = size >> 1; stride > 0; stride >>= 1) warp_step(k, first, size, stride, lane);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) list[first + r * 32 + lane] = k[r];
+    }
     __syncthreads();
-    block_bitonic_desc(list, P);
+    for (int size = 256; size <= P; size <<= 1) {
+        for (int stride = size >> 1; stride >= 128; stride >>= 1) {
+            for (int q = threadIdx.x; q < (P >> 1); q += NT) {
+                const int i = 2 * stride * (q / stride) + (q % stride), l = i + stride;
+                const u64 x = list[i], y = list[l];
+                if (((i & size) == 0) ? (x < y) : (x > y)) {
+                    list[i] = y;
+                    list[l] = x;
+                }
+            }
+            __syncthreads();
+        }
+        for (int first = warp * 128; first < P; first += NT / 32 * 128) {
+            u64 k[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) k[r] = list[first + r * 32 + lane];
+#pragma unroll
+            for (int stride = 64; stride > 0; stride >>= 1) warp_step(k, first, size, stride, lane);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) list[first + r * 32 + lane] = k[r];
+        }
+        __syncthreads();
+    }
 }
 
 // cum[i] = base + the mass of the sorted entries 0 .. i.
 template <int NT>
-__device__ void scan_list(const u64* list, double* cum, int n, double base, float top, double temperature,
-                          FastSmem<NT>& sm) {
-    constexpr int R = kListCap / NT > 0 ? kListCap / NT : 1;
+__device__ void scan_list(const u64* list, double* cum, int n, double base, const RowFacts& f, FastSmem<NT>& sm) {
+    constexpr int R = (kListCap + NT - 1) / NT;
     double w[R], t = 0.0;
 #pragma unroll
     for (int j = 0; j < R; ++j) {
         const int i = (int)threadIdx.x * R + j;
-        w[j] = i < n ? weight64(key_value((uint32_t)(list[i] >> 32)), top, temperature) : 0.0;
+        w[j] = i < n ? f.weight(key_value((uint32_t)(list[i] >> 32))) : 0.0;
         t += w[j];
     }
-    double c = base + block_scan<NT>(t, sm.red_d) - t;
+    double c = base + (block_scan<NT>(t, sm.red_d) - t);
 #pragma unroll
     for (int j = 0; j < R; ++j) {
         const int i = (int)threadIdx.x * R + j;
@@ -623,6 +785,25 @@ __device__ void scan_list(const u64* list, double* cum, int n, double base, floa
         if (i < n) cum[i] = c;
     }
     __syncthreads();
+}
+
+// The same two for a list of up to kWarpList keys, by one warp.
+__device__ __forceinline__ void sort_and_scan_warp(u64* list, double* cum, int n, const RowFacts& f, int lane) {
+    if (n <= 32) warp_sort_desc<1>(list, n, lane);
+    else warp_sort_desc<kWarpList / 32>(list, n, lane);
+    __syncwarp();
+    double before = 0.0;
+    for (int i = lane; i - lane < n; i += 32) {
+        double c = i < n ? f.weight(key_value((uint32_t)(list[i] >> 32))) : 0.0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const double u = __shfl_up_sync(kFullMask, c, o);
+            if (lane >= o) c += u;
+        }
+        if (i < n) cum[i] = before + c;
+        before += __shfl_sync(kFullMask, c, 31);
+    }
+    __syncwarp();
 }
 
 // Number of leading entries with cum <= bound, by one warp.
@@ -637,36 +818,36 @@ __device__ __forceinline__ int count_below(const double* cum, int n, double boun
     return c;
 }
 
-__device__ __forceinline__ void write_row(const FilterLaunch& p, int r, int id, float x, float top, double temperature,
-                                          double total, int kept) {
-    p.out_ids[r] = id;
-    if (p.logprobs)
-        p.logprobs[r] = (float)((x == top ? 0.0 : ((double)x - (double)top) / temperature) - log(total));
+__device__ __forceinline__ void write_row(const FilterLaunch& p, int r, u64 key, const RowFacts& f, double total,
+                                          int kept) {
+    p.out_ids[r] = key_index(key);
+    if (p.logprobs) {
+        const double d = ((double)key_value((uint32_t)(key >> 32)) - (double)f.top) * f.z64;
+        const float t = (float)total;  // ln in fp32 plus what the rounding of its argument left
+        p.logprobs[r] = (float)(d * 0.69314718055994530942 - ((double)logf(t) + (total - (double)t) / (double)t));
+    }
     if (p.kept) p.kept[r] = kept;
     if (p.row_flags) p.row_flags[r] = 0;
 }
 
-// Passes 2: the threshold and the list above it.  kNeedBins when the list
-// would not hold it, kNeedSum64 when it is there but the bound of f.sum's error
-// spans a border (then sum_is64 says that `sum` is exact).
+// Decides a row by its sorted list, by one warp.  kNeedBins when the list does
+// not reach far enough, kNeedSum64 when `sum`, off by up to err, leaves a border
+// open.  `complete`: every candidate is listed.
 template <int NT>
 __device__ int decide_list(const FilterLaunch& p, int r, const RowRule& rule, const RowFacts& f, int n, bool complete,
                            int k, double sum, double err, int candidates, FastSmem<NT>& sm) {
-    // one warp
     const int lane = threadIdx.x & 31;
-    const double temperature = (double)rule.temperature;
     const u64* key = sm.list.key;
     const double* cum = sm.list.cum;
-    const bool limited = k > 0 || rule.minp > 0.0f || complete;
     const bool use_p = rule.topp > 0.0f && rule.topp < 1.0f;
+    const bool listed = k > 0 || rule.minp > 0.0f || complete;  // the mass that top-p and the draw refer to
     int kept = n;
-    double lo = sum * (1.0 - err), hi = sum * (1.0 + err);
-    if (limited) {
+    double lo = sum - err, hi = sum + err;
+    if (listed) {
         if (rule.minp > 0.0f) {
-            int c = 0;
+            kept = 0;
             for (int i = lane; i - lane < n; i += 32)
-                c += __popc(__ballot_sync(kFullMask, i < n && key_value((uint32_t)(key[i] >> 32)) >= f.minp_at));
-            kept = c;
+                kept += __popc(__ballot_sync(kFullMask, i < n && key_value((uint32_t)(key[i] >> 32)) >= f.minp_at));
         }
         if (k > 0 && k < kept) kept = k;
         if (kept < 1) return kNeedExact;
@@ -674,160 +855,146 @@ __device__ int decide_list(const FilterLaunch& p, int r, const RowRule& rule, co
     }
     if (use_p) {
         const int at = count_below(cum, kept, (double)rule.topp * lo) + 1;
-        if (!limited) {
+        if (!listed) {
             if (at > n) return kNeedBins;
             if (count_below(cum, n, (double)rule.topp * hi) + 1 != at) return kNeedSum64;
         }
         kept = min(kept, at);
         lo = hi = cum[kept - 1];
     }
-    int at = count_below(cum, limited || use_p ? kept : n, (double)rule.coin * lo);
-    if (!limited && !use_p) {
+    int at = count_below(cum, kept, (double)rule.coin * lo);
+    if (!listed && !use_p) {
         if (at >= n) return kNeedBins;
         if (count_below(cum, n, (double)rule.coin * hi) != at) return kNeedSum64;
         kept = candidates;
         lo = sum;
-    } else if (at > kept - 1) {
-        at = kept - 1;
     }
-    if (lane == 0)
-        write_row(p, r, key_index(key[at]), key_value((uint32_t)(key[at] >> 32)), f.top, temperature, lo, kept);
+    at = min(at, kept - 1);
+    if (lane == 0) write_row(p, r, key[at], f, lo, kept);
     return kDone;
 }
 
+// Pass 2: a threshold below which nothing can be kept or drawn, and the row
+// decided by the list of the entries above it.
 template <int NT, typename T>
-__device__ int sample_from_list(const FilterLaunch& p, int r, const VecRow<T>& row, const RowRule& rule,
-                                const RowFacts& f, int k, FastSmem<NT>& sm) {
+__device__ __forceinline__ int sample_from_list(const FilterLaunch& p, int r, const VecRow<T>& row, const RowRule& rule,
+                                                const RowFacts& f, int k, FastSmem<NT>& sm) {
     constexpr int E = VecRow<T>::E;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const float inf = __int_as_float(0x7F800000);
     const bool use_p = rule.topp > 0.0f && rule.topp < 1.0f;
-    const double temperature = (double)rule.temperature;
-    float cut = -inf;
-    if (row.vocab > kListCap) {
-        // chunk maxima over [low_chunk, top]: how many chunks, and how much mass in
-        // their maxima alone, lie at or above each bin's lower edge
-        const float span = f.top - f.low_chunk;
-        const float scale = span > 0.0f ? (float)(kChunkBins - 1) / span : 0.0f;
-        for (int i = threadIdx.x; i < kChunkBins; i += NT) sm.hist.mass[i] = sm.hist.count[i] = 0u;
-        __syncthreads();
+    // neither top-k nor min-p: the mass is the row's
+    const bool open = k == 0 && !(rule.minp > 0.0f);
+    // chunk maxima over [low_chunk, top]: how many, and how much mass in them alone,
+    // lie at or above each bin's lower edge.  Bin b is at 32 * (b % 16) + b / 16, so
+    // that the lanes of the scan, 16 bins each, read 32 banks.
+    const float span = f.top - f.low_chunk;
+    const float scale = span > 0.0f ? (float)(kChunkBins - 1) / span : 0.0f;
+    if (open || k > 0) {
         for (int i = threadIdx.x; i < f.chunks; i += NT) {
             const float m = sm.chunk_max[i];
             if (m > -inf) {
                 const int b = min((int)((f.top - m) * scale), kChunkBins - 1);
-                atomicAdd(&sm.hist.count[b], 1u);
-                atomicAdd(&sm.hist.mass[b], (unsigned)(ex2_approx((m - f.top) * f.z) * 0x1p20f));
+                const int at = ((b & 15) << 5) | (b >> 4);
+                atomicAdd(&sm.chunk_bin[at], k > 0 ? 1u : (unsigned)(ex2_approx((m - f.top) * f.z) * 0x1p20f));
             }
         }
         __syncthreads();
-        if (warp == 0) {
-            constexpr int R = kChunkBins / 32;
-            unsigned c = 0, w = 0;
+    }
+    // every warp forms the same threshold
+    float cut = -inf;
+    if (open || k > 0) {
+        constexpr int R = kChunkBins / 32;
+        unsigned v[R], c = 0;
 #pragma unroll
-            for (int j = 0; j < R; ++j) {
-                c += sm.hist.count[lane * R + j];
-                w += sm.hist.mass[lane * R + j];
-            }
-            unsigned ci = c, wi = w;
+        for (int j = 0; j < R; ++j) c += v[j] = sm.chunk_bin[j * 32 + lane];
+        unsigned ci = c;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const unsigned cu = __shfl_up_sync(kFullMask, ci, o), wu = __shfl_up_sync(kFullMask, wi, o);
-                if (lane >= o) {
-                    ci += cu;
-                    wi += wu;
-                }
-            }
-            ci -= c;
-            wi -= w;
-            // the first bin by which the chunk maxima alone hold k entries, or the mass asked for
-            const float part = use_p ? rule.topp : rule.coin;
-            const float want = part * (float)f.sum * 1.0001f * 0x1p20f + (float)f.chunks;
-            int found = kChunkBins;
-#pragma unroll
-            for (int j = 0; j < R; ++j) {
-                ci += sm.hist.count[lane * R + j];
-                wi += sm.hist.mass[lane * R + j];
-                const bool there = k > 0 ? ci >= (unsigned)k : (float)wi >= want;
-                if (there && found == kChunkBins) found = lane * R + j;
-            }
-            const unsigned who = __ballot_sync(kFullMask, found < kChunkBins);
-            found = __shfl_sync(kFullMask, found, who ? __ffs(who) - 1 : 31);
-            float t = found < kChunkBins ? __fsub_rd(f.top, ((float)found + 1.01f) / scale) : -inf;
-            if (found < kChunkBins && !(span > 0.0f)) t = f.top;
-            if (k == 0 && !(rule.minp > 0.0f)) {
-                // what lies below this cannot hold the rest of the mass, however many they are
-                const float rest = fmaxf(1.0f - part, 0x1p-24f) * (float)f.sum;
-                const float skip = __fsub_rd(f.top, 1.001f * __log2f(1.01f * (float)row.vocab / rest) / f.z);
-                if (skip > t) t = skip;
-            }
-            if (rule.minp > 0.0f) t = k > 0 ? fmaxf(t, f.minp_at) : f.minp_at;
-            // chunks that hold entries above the threshold
-            unsigned hit = 0;
-            for (int i = lane; i < f.chunks; i += 32) hit += sm.chunk_max[i] >= t;
-            hit = __reduce_add_sync(kFullMask, hit);
-            // entries to expect, were they spread over the chunks at random
-            const float g = (float)f.chunks;
-            const float expect = (float)hit < g ? -g * __logf(1.0f - (float)hit / g) : 1e9f;
-            if (lane == 0) {
-                sm.red_f[0][0] = t;
-                sm.status = expect <= 0.9f * kListCap ? kDone : kNeedBins;
-                sm.n[0] = 0u;
-            }
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned cu = __shfl_up_sync(kFullMask, ci, o);
+            if (lane >= o) ci += cu;
         }
-        __syncthreads();
-        if (sm.status != kDone) return kNeedBins;
-        cut = sm.red_f[0][0];
-    } else if (threadIdx.x == 0) {
-        sm.n[0] = 0u;
+        ci -= c;
+        // the first bin by which the chunk maxima alone hold k entries, or the mass asked for
+        const float part = use_p ? rule.topp : rule.coin;
+        const float want = k > 0 ? (float)k : part * f.sum * 1.0001f * 0x1p20f + (float)f.chunks;
+        int found = kChunkBins;
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            ci += v[j];
+            if ((float)ci >= want && found == kChunkBins) found = lane * R + j;
+        }
+        found = __reduce_min_sync(kFullMask, found);
+        if (found < kChunkBins) cut = span > 0.0f ? __fsub_rd(f.top, ((float)found + 1.01f) / scale) : f.top;
+        if (open) {
+            // what lies below this cannot hold the rest of the mass, however many they are
+            const float rest = fmaxf(1.0f - part, 0x1p-24f) * f.sum;
+            cut = fmaxf(cut, __fsub_rd(f.top, 1.001f * __log2f(1.01f * (float)row.vocab / rest) / f.z));
+        }
+    }
+    if (rule.minp > 0.0f) cut = fmaxf(cut, f.minp_at);
+    // chunks that hold entries above the threshold
+    for (int c = threadIdx.x; c < f.chunks; c += NT) {
+        const bool hit = sm.chunk_max[c] >= cut;
+        const unsigned who = __ballot_sync(kFullMask, hit);
+        if (who == 0u) continue;
+        unsigned at = 0;
+        if (lane == 0) at = atomicAdd(&sm.hits, (unsigned)__popc(who));
+        at = __shfl_sync(kFullMask, at, 0) + __popc(who & ((1u << lane) - 1u));
+        if (hit) sm.list.hit[at] = c;
     }
     __syncthreads();
-    // the entries at or above the threshold
+    int hits = (int)sm.hits;
+    // entries to expect, were they spread over the chunks at random
+    const float g = (float)f.chunks;
+    const float expect = hits < f.chunks ? -g * __logf(1.0f - (float)hits / g) : 1e9f;
+    if (row.vocab <= kListCap && expect > 0.3f * kListCap) {
+        cut = -inf;
+        hits = f.chunks;
+        __syncthreads();
+        for (int c = threadIdx.x; c < f.chunks; c += NT) sm.list.hit[c] = c;
+        __syncthreads();
+    } else if (expect > 0.9f * kListCap) {
+        return kNeedBins;
+    }
     const bool complete = !(cut > -inf);
-    const int strips = (row.vecs + 31) >> 5;
-    for (int c0 = warp * 32; c0 < f.chunks; c0 += NT) {
-        unsigned todo = __ballot_sync(kFullMask, c0 + lane < f.chunks && sm.chunk_max[c0 + lane] >= cut);
-        while (todo) {
-            float v[kInFlight][E];
-            int strip[kInFlight];
-            if (f.chunk_shift == 0) {
+    for (int i = threadIdx.x; i < hits; i += NT) {
+        const int c = sm.list.hit[i];
+        for (int j = 0; j <= (1 << f.chunk_shift) - 1; ++j) {
+            const int first = ((((c >> 5) << f.chunk_shift) + j) * kU << 5) | (c & 31);
+            uint4 raw[kU];
 #pragma unroll
-                for (int u = 0; u < kInFlight; ++u) {
-                    strip[u] = todo ? c0 + __ffs(todo) - 1 : strips;
-                    todo &= todo - 1;
-                }
-            } else {
-                const int s0 = (c0 + __ffs(todo) - 1) << 2;
-                todo &= todo - 1;
+            for (int u = 0; u < kU; ++u) raw[u] = row.load(first + 32 * u);
 #pragma unroll
-                for (int u = 0; u < kInFlight; ++u) strip[u] = s0 + u;
-            }
-#pragma unroll
-            for (int u = 0; u < kInFlight; ++u) row.load(strip[u] * 32 + lane, v[u]);
-#pragma unroll
-            for (int u = 0; u < kInFlight; ++u) {
+            for (int u = 0; u < kU; ++u) {
+                float v[E];
+                VecRow<T>::widen(raw[u], v);
                 unsigned mask = 0u;
 #pragma unroll
-                for (int e = 0; e < E; ++e) mask |= (v[u][e] >= cut && v[u][e] > -inf) ? 1u << e : 0u;
-                push_entries<T>(row, strip[u] * 32 + lane, v[u], mask, sm.list.key, kListCap, &sm.n[0]);
+                for (int e = 0; e < E; ++e) mask |= (v[e] >= cut && v[e] > -inf) ? 1u << e : 0u;
+                push_entries<T>(row, first + 32 * u, v, mask, sm.list.key, kListCap, &sm.n[0]);
             }
         }
     }
     __syncthreads();
     const int n = (int)sm.n[0];
     const bool all_of_minp = rule.minp > 0.0f && cut <= f.minp_at;
-    if (n > kListCap || (k > 0 && n < k && !complete && !all_of_minp) || n < 1) return kNeedBins;
-    sort_list<NT>(sm.list.key, n);
-    scan_list<NT>(sm.list.key, sm.list.cum, n, 0.0, f.top, temperature, sm);
+    if (n > kListCap || n < 1 || (k > 0 && n < k && !complete && !all_of_minp)) return kNeedBins;
     int candidates = row.vocab;
-    if (!(f.low > -inf) && k == 0 && !(rule.minp > 0.0f) && !use_p && !complete && p.kept)
-        candidates = count_candidates<NT>(row, sm);
+    if (open && !use_p && !complete && !(f.low > -inf) && p.kept) candidates = count_candidates<NT>(row, sm);
+    if (n > kWarpList) {
+        sort_list<NT>(sm.list.key, n);
+        scan_list<NT>(sm.list.key, sm.list.cum, n, 0.0, f, sm);
+    }
     if (warp == 0) {
-        const int st = decide_list<NT>(p, r, rule, f, n, complete, k, f.sum, f.sum_err, candidates, sm);
+        if (n <= kWarpList) sort_and_scan_warp(sm.list.key, sm.list.cum, n, f, lane);
+        const int st = decide_list<NT>(p, r, rule, f, n, complete, k, (double)f.sum, (double)f.sum * f.sum_err,
+                                       candidates, sm);
         if (lane == 0) sm.status = st;
     }
     __syncthreads();
     if (sm.status != kNeedSum64) return sm.status;
-    const double s64 = sum64<NT>(row, f.top, temperature, 0ull, sm);
+    const double s64 = sum64<NT>(row, f, sm);
     if (warp == 0) {
         const int st = decide_list<NT>(p, r, rule, f, n, complete, k, s64, 0.0, candidates, sm);
         if (lane == 0) sm.status = st;
@@ -837,71 +1004,62 @@ __device__ int sample_from_list(const FilterLaunch& p, int r, const VecRow<T>& r
 }
 
 // ---- flat rows ----------------------------------------------------------------
-// Coordinates of the bins: (top - x) * scale, rising as the logit falls.
-struct BinScale {
-    float top, scale, z;
-    __device__ __forceinline__ float at(float x) const { return (top - x) * scale; }
-    __device__ __forceinline__ float weight(float x) const { return ex2_approx((x - top) * z); }
+struct Bracket {
+    float lo, hi;   // bin coordinates [lo, hi) of the bins that hold the crossing; "above" is below lo
+    double mass;    // of the entries above
+    int above;      // their number
+    int n;          // entries in the bracket's list
 };
 
-// Histogram of count or mass of the entries >= low, and their mass and number.
-// mass_unit: units of the mass histogram per weight.
+// Coordinates of the bins: (top - x) * scale, rising as the logit falls.
+struct BinScale {
+    float top, scale;
+    __device__ __forceinline__ float at(float x) const { return (top - x) * scale; }
+};
+
+// Histogram of the count (kCount) or of the fp32 mass, in `unit`s, of the
+// entries >= low that have a bin, and the number of all entries >= low.
 template <int NT, typename T, bool kCount>
-__device__ void fill_bins(const VecRow<T>& row, const BinScale& b, float low, float mass_unit, double& mass, int& number,
-                          FastSmem<NT>& sm) {
+__device__ __forceinline__ int fill_bins(const VecRow<T>& row, const BinScale& b, float z, float low, float unit,
+                                         FastSmem<NT>& sm) {
     constexpr int E = VecRow<T>::E;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int strips = (row.vecs + 31) >> 5;
-    unsigned* hist = kCount ? sm.hist.count : sm.hist.mass;
+    unsigned* hist = sm.hist.bin;
     for (int i = threadIdx.x; i < kBinCap; i += NT) hist[i] = 0u;
     __syncthreads();
-    double s = 0.0;
-    int c = 0;
-    for (int s0 = warp * kInFlight; s0 < strips; s0 += (NT / 32) * kInFlight) {
-        float v[kInFlight][E];
+    unsigned c = 0;
+    for (int i = warp; i < row.batches; i += NT / 32) {
+        uint4 raw[kU];
+        row.load_batch(i, lane, raw);
 #pragma unroll
-        for (int u = 0; u < kInFlight; ++u) row.load((s0 + u) * 32 + lane, v[u]);
-        float t[kInFlight];
-#pragma unroll
-        for (int u = 0; u < kInFlight; ++u) {
+        for (int u = 0; u < kU; ++u) {
+            float v[E];
+            VecRow<T>::widen(raw[u], v);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                const float x = v[u][e];
-                const bool in = x >= low;
-                const int bin = min((int)b.at(x), kBinCap - 1);
-                if (kCount) {
-                    if (in) atomicAdd(&hist[bin], 1u);
-                } else {
-                    const float w = in ? b.weight(x) : 0.0f;
-                    if (in) atomicAdd(&hist[bin], __float2uint_rn(w * mass_unit));
-                    v[u][e] = w;
-                }
+                const bool in = v[e] >= low;
+                const float at = b.at(v[e]);
                 c += in;
+                if (in && at < (float)kBinCap)
+                    atomicAdd(&hist[(int)at], kCount ? 1u : __float2uint_rn(ex2_approx((v[e] - b.top) * z) * unit));
             }
-            t[u] = kCount ? 0.0f : tree_sum(v[u]);
         }
-        if (!kCount) s += (double)tree_sum(t);
     }
-    mass = kCount ? 0.0 : block_sum<NT>(s, sm.red_d);
-    number = (int)block_sum<NT>((double)c, sm.red_d);
+    return (int)block_sum<NT>(c, sm.red_u);
 }
 
-// First bins whose inclusive running sum exceeds each bound (kBinCap: none).
+// First bins whose inclusive running sum exceeds each bound (kBinCap: none; 0 for a bound below 0).
 template <int NT>
-__device__ void locate(const unsigned* hist, const float (&bound)[4], int (&bin)[4], FastSmem<NT>& sm) {
+__device__ __forceinline__ void locate(const float (&bound)[4], int (&bin)[4], FastSmem<NT>& sm) {
     constexpr int R = kBinCap / NT;
+    const unsigned* hist = sm.hist.bin;
     if (threadIdx.x < 4) sm.bin[threadIdx.x] = kBinCap;
-    unsigned v[R], t = 0;
-#pragma unroll
-    for (int j = 0; j < R; ++j) {
-        v[j] = hist[threadIdx.x * R + j];
-        t += v[j];
-    }
-    unsigned c = block_scan<NT>(t, sm.red_u[0]) - t;
-#pragma unroll
+    unsigned t = 0;
+    for (int j = 0; j < R; ++j) t += hist[threadIdx.x * R + j];
+    unsigned c = block_scan<NT>(t, sm.red_u) - t;
     for (int j = 0; j < R; ++j) {
         const float before = (float)c;
-        c += v[j];
+        c += hist[threadIdx.x * R + j];
 #pragma unroll
         for (int q = 0; q < 4; ++q)
             if ((float)c > bound[q] && before <= bound[q]) atomicMin(&sm.bin[q], (int)threadIdx.x * R + j);
@@ -912,93 +1070,96 @@ __device__ void locate(const unsigned* hist, const float (&bound)[4], int (&bin)
     __syncthreads();
 }
 
-// The entries of two brackets (half the list each) and the mass and number above
-// them.
-template <int NT, typename T, bool kDouble>
-__device__ void gather_brackets(const VecRow<T>& row, const BinScale& b, float low, double temperature,
-                                Bracket (&br)[2], FastSmem<NT>& sm) {
+// The entries of two brackets (list 1 from `split` on) and, with kMass, the
+// masses in fp64: above each bracket and in all.  Entries below `low`, and
+// those that equal it with an index above `last`, are not seen.  Returns the
+// mass of all.
+template <int NT, typename T, bool kMass>
+__device__ __forceinline__ double gather_brackets(const VecRow<T>& row, const RowFacts& f, const BinScale& b, float low,
+                                                  int last, int split, Bracket (&br)[2], FastSmem<NT>& sm) {
     constexpr int E = VecRow<T>::E;
-    constexpr int U = kInFlight;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int strips = (row.vecs + 31) >> 5;
+    const double c = -(double)f.top * f.z64;
     if (threadIdx.x < 2) sm.n[threadIdx.x] = 0u;
     __syncthreads();
-    double mass[2] = {0.0, 0.0};
-    int above[2] = {0, 0};
-    for (int s0 = warp * U; s0 < strips; s0 += (NT / 32) * U) {
-        float v[U][E], t[2][U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) row.load((s0 + u) * 32 + lane, v[u]);
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            float w[2][E];
-            unsigned mask[2] = {0u, 0u};
+    double all = 0.0, mass[2] = {0.0, 0.0};
+    unsigned above = 0;
+    for (int i = warp; i < row.batches; i += NT / 32) {
+        uint4 raw[kU];
+        row.load_batch(i, lane, raw);
+#pragma unroll 1
+        for (int u = 0; u < kU; ++u) {
+            const int vec = (i * kU + u) * 32 + lane;
+            float v[E];
+            uint4 w = raw[0];
+            if (u == 1) w = raw[1];
+            if (u == 2) w = raw[2];
+            if (u == 3) w = raw[3];
+            VecRow<T>::widen(w, v);
+            unsigned mask0 = 0u, mask1 = 0u;
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                const float x = v[u][e], at = b.at(x);
-                const bool in = x >= low;
-                const float m = kDouble ? 0.0f : b.weight(x);
-#pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    const bool a = in && at < br[q].lo;
-                    above[q] += a;
-                    w[q][e] = a ? m : 0.0f;
-                    mask[q] |= (in && !a && at < br[q].hi) ? 1u << e : 0u;
-                    if (kDouble && a) mass[q] += weight64(x, b.top, temperature);
+                const float at = b.at(v[e]);
+                bool in = v[e] >= low;
+                if (v[e] == low && row.index(vec, e) > last) in = false;
+                const bool a0 = in && at < br[0].lo, a1 = in && at < br[1].lo;
+                above += a0;
+                mask0 |= (in && !a0 && at < br[0].hi) ? 1u << e : 0u;
+                mask1 |= (in && !a1 && at < br[1].hi) ? 1u << e : 0u;
+                if (kMass) {
+                    const double m = in ? exp2_64(fma((double)v[e], f.z64, c)) : 0.0;
+                    all += m;
+                    mass[0] += a0 ? m : 0.0;
+                    mass[1] += a1 ? m : 0.0;
                 }
             }
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                t[q][u] = tree_sum(w[q]);
-                push_entries<T>(row, (s0 + u) * 32 + lane, v[u], mask[q], sm.list.key + q * (kListCap / 2),
-                                kListCap / 2, &sm.n[q]);
-            }
-        }
-        if (!kDouble) {
-            mass[0] += (double)tree_sum(t[0]);
-            mass[1] += (double)tree_sum(t[1]);
+            push_entries<T>(row, vec, v, mask0, sm.list.key, split, &sm.n[0]);
+            push_entries<T>(row, vec, v, mask1, sm.list.key + split, kListCap - split, &sm.n[1]);
         }
     }
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-        br[q].mass = block_sum<NT>(mass[q], sm.red_d);
-        br[q].above = (int)block_sum<NT>((double)above[q], sm.red_d);
-        br[q].n = (int)sm.n[q];
+    br[0].above = (int)block_sum<NT>(above, sm.red_u);
+    if (kMass) {
+        all = block_sum<NT>(all, sm.red_d);
+        br[0].mass = block_sum<NT>(mass[0], sm.red_d);
+        br[1].mass = block_sum<NT>(mass[1], sm.red_d);
     }
+    br[0].n = (int)sm.n[0];
+    br[1].n = (int)sm.n[1];
+    return all;
 }
 
+// Pass 3: the crossings by histogram.  Brackets are first as narrow as the
+// histogram's typical error makes them, then as wide as its largest.
 template <int NT, typename T>
 __device__ __noinline__ int sample_by_bins(const FilterLaunch& p, int r, const VecRow<T>& row, const RowRule& rule,
                                            const RowFacts& f, int k, FastSmem<NT>& sm) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const float inf = __int_as_float(0x7F800000);
     const bool use_p = rule.topp > 0.0f && rule.topp < 1.0f;
-    const double temperature = (double)rule.temperature;
-    float low = rule.minp > 0.0f ? f.minp_at : -3.402823466e38f;  // logits below it are out
-    u64 limit = 0;                                                // and so are keys below this
-    BinScale b{f.top, 0.0f, f.z};
+    float low = rule.minp > 0.0f ? f.minp_at : kLowest;  // logits below it are out,
+    int last = 0x7FFFFFFF;                               // and so are equal ones with a larger index
+    BinScale b{f.top, 0.0f};
     const Bracket none{0.0f, 0.0f, 0.0, 0, 0};
-    const auto past = [&](int bin) { return bin + 1 < kBinCap ? (float)(bin + 1) : inf; };  // the last bin has no end
-    double sum;
-    int number;
+    int number = 0;
     if (k > 0) {
         // top-k: the k-th entry in the order
-        const float floor_at = fmaxf(fmaxf(low, f.low), f.low_chunk - 2.0f * (f.top - f.low_chunk));
-        const float span = f.top - floor_at;
+        const float span = f.top - fmaxf(fmaxf(low, f.low), f.low_chunk - 2.0f * (f.top - f.low_chunk));
         if (!(span > 0.0f) || !(span < 1e37f)) return kNeedExact;
         b.scale = (float)(kBinCap - 1) / span;
-        fill_bins<NT, T, true>(row, b, low, 0.0f, sum, number, sm);
+        number = fill_bins<NT, T, true>(row, b, f.z, low, 0.0f, sm);
         if (number > k) {
             const float bound[4] = {(float)(k - 1), -1.0f, -1.0f, -1.0f};  // k <= 2^20: exact
             int bin[4];
-            locate<NT>(sm.hist.count, bound, bin, sm);
-            Bracket br[2] = {{(float)bin[0], past(bin[0]), 0.0, 0, 0}, none};
-            gather_brackets<NT, T, false>(row, b, low, temperature, br, sm);
+            locate<NT>(bound, bin, sm);
+            if (bin[0] >= kBinCap) return kNeedExact;
+            Bracket br[2] = {{(float)bin[0], (float)(bin[0] + 1), 0.0, 0, 0}, none};
+            gather_brackets<NT, T, false>(row, f, b, low, last, kListCap, br, sm);
             const int at = k - 1 - br[0].above;
-            if (br[0].n > kListCap / 2 || at < 0 || at >= br[0].n) return kNeedExact;
+            if (br[0].n > kListCap || at < 0 || at >= br[0].n) return kNeedExact;
             sort_list<NT>(sm.list.key, br[0].n);
-            limit = sm.list.key[at];
-            low = key_value((uint32_t)(limit >> 32));
+            low = key_value((uint32_t)(sm.list.key[at] >> 32));
+            last = key_index(sm.list.key[at]);
+            number = k;
             __syncthreads();
         } else {
             k = 0;
@@ -1010,110 +1171,106 @@ __device__ __noinline__ int sample_by_bins(const FilterLaunch& p, int r, const V
     {
         float bits = 48.0f;
         if (!limited) {
-            const float rest = fmaxf(1.0f - (use_p ? rule.topp : rule.coin), 0x1p-24f) * (float)f.sum;
+            const float rest = fmaxf(1.0f - (use_p ? rule.topp : rule.coin), 0x1p-24f) * f.sum;
             bits = fminf(bits, 1.001f * __log2f(1.01f * (float)row.vocab / rest));
         }
         const float span = f.top - fmaxf(f.top - bits / f.z, fmaxf(low, f.low));
         if (!(span < 1e37f)) return kNeedExact;
         b.scale = span > 0.0f ? (float)(kBinCap - 1) / span : 0.0f;
     }
-    const float unit = 0x1p30f / (1.001f * (float)f.sum);
-    fill_bins<NT, T, false>(row, b, low, unit, sum, number, sm);
-    double err = f.sum_err * f.sum;  // of `sum` and of the masses above the brackets alike
-    if (!limited) sum = f.sum;
-    if (k > 0) number = k;
-    // bins are off by half a unit an entry and by the weights' error
-    const float slack = 0.5f * (float)row.vocab + 0x1p30f * 2e-5f;
-    const float t = (use_p ? rule.topp : 1.0f) * (float)sum * unit, u = rule.coin * t;
-    float bound[4] = {t - slack, t + slack, u - slack, -1.0f};
-    int bin[4];
-    locate<NT>(sm.hist.mass, bound, bin, sm);
-    Bracket br[2] = {none, none};
-    if (use_p) {
-        if (bin[0] >= kBinCap) return kNeedExact;
-        br[0].lo = (float)bin[0];
-        br[0].hi = past(bin[1]);
-        // what is kept weighs up to one crossing's bins more than top-p asks for
-        bound[0] = u + slack + rule.coin * ((float)sm.hist.mass[bin[0]] + (float)sm.hist.mass[min(bin[1], kBinCap - 1)]);
-    } else {
-        bound[0] = u + slack;
-    }
-    if (bin[2] >= kBinCap) return kNeedExact;
-    br[1].lo = (float)bin[2];
-    __syncthreads();
-    bound[1] = bound[2] = -1.0f;
-    locate<NT>(sm.hist.mass, bound, bin, sm);
-    br[1].hi = past(bin[0]);
-    for (int precise = k > 0 ? 1 : 0; precise < 2; ++precise) {
-        if (precise) {  // entries that equal the k-th and come after it are in the fp32 sum
-            sum = sum64<NT>(row, f.top, temperature, k > 0 ? limit : limited ? (u64)order_key(low) << 32 : 0ull, sm);
-            err = 0.0;
-            gather_brackets<NT, T, true>(row, b, low, temperature, br, sm);
-        } else {
-            gather_brackets<NT, T, false>(row, b, low, temperature, br, sm);
+    const int split = use_p ? kListCap / 2 : 0;
+    const float unit = 0x1p30f / (1.001f * f.sum);
+    double limited_sum = -1.0;
+    for (int wide = 0; wide < 2; ++wide) {
+        const int counted = fill_bins<NT, T, false>(row, b, f.z, low, unit, sm);
+        if (k == 0) number = counted;
+        // an entry is off by up to half a unit, at random by a third; the weights by
+        // 2e-5 at most
+        const float slack = wide ? 0.5f * (float)row.vocab + 0x1p30f * 2e-5f
+                                 : 3.0f * sqrtf((float)row.vocab) + 0x1p30f * 1e-6f;
+        float total_units = f.sum * unit;
+        if (limited && limited_sum < 0.0) {
+            unsigned t = 0;
+            for (int i = threadIdx.x; i < kBinCap; i += NT) t += sm.hist.bin[i];
+            total_units = (float)block_sum<NT>(t, sm.red_u);
+        } else if (limited) {
+            total_units = (float)limited_sum * unit;
         }
-        if (br[0].n > kListCap / 2 || br[1].n > kListCap / 2) return kNeedExact;
-        u64* const list[2] = {sm.list.key, sm.list.key + kListCap / 2};
-        double* const cum[2] = {sm.list.cum, sm.list.cum + kListCap / 2};
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
+        const float t = (use_p ? rule.topp : 1.0f) * total_units, u = rule.coin * t;
+        float bound[4] = {t - slack, t + slack, u - slack, -1.0f};
+        int bin[4];
+        locate<NT>(bound, bin, sm);
+        Bracket br[2] = {none, none};
+        const auto past = [&](int q) { return q < kBinCap ? (float)(q + 1) : inf; };
+        if (bin[2] >= kBinCap || (use_p && bin[0] >= kBinCap)) return kNeedExact;
+        bound[0] = u + slack;
+        if (use_p) {
+            br[0].lo = (float)bin[0];
+            br[0].hi = past(bin[1]);
+            // what is kept weighs up to one crossing's bins more than top-p asks for
+            bound[0] += rule.coin * ((float)sm.hist.bin[bin[0]] + (float)sm.hist.bin[min(bin[1], kBinCap - 1)]);
+        }
+        br[1].lo = (float)bin[2];
+        bound[1] = bound[2] = -1.0f;
+        __syncthreads();
+        locate<NT>(bound, bin, sm);
+        br[1].hi = past(bin[0]);
+        const double sum = gather_brackets<NT, T, true>(row, f, b, low, last, split, br, sm);
+        if (br[0].n > split || br[1].n > kListCap - split) return kNeedExact;
+        u64* const list[2] = {sm.list.key, sm.list.key + split};
+        double* const cum[2] = {sm.list.cum, sm.list.cum + split};
+#pragma unroll 1
+        for (int q = use_p ? 0 : 1; q < 2; ++q) {
             sort_list<NT>(list[q], br[q].n);
-            scan_list<NT>(list[q], cum[q], br[q].n, br[q].mass, f.top, temperature, sm);
+            scan_list<NT>(list[q], cum[q], br[q].n, br[q].mass, f, sm);
         }
         if (warp == 0) {
-            // place of the crossing of `bnd` in bracket q, where `border` bounds the error of
-            // the difference between the bound and a running mass
-            const auto place = [&](int q, double bnd, double border, int& st) {
-                const int lo = count_below(cum[q], br[q].n, bnd - border), hi = count_below(cum[q], br[q].n, bnd + border);
-                if (br[q].mass > bnd + border || lo >= br[q].n) st = kNeedExact;  // not in this bracket
-                else if (lo != hi || (br[q].above > 0 && br[q].mass > bnd - border)) st = kNeedSum64;
-                return lo;
-            };
             int st = kDone, kept = number;
             double total = sum;
             if (use_p) {
-                const int at = place(0, (double)rule.topp * sum, 2.0 * err, st);
-                if (st == kDone) {
-                    kept = min(br[0].above + at + 1, number);  // equals of the k-th behind it are not kept
-                    const int last = kept - 1 - br[0].above;
-                    if (last < 0) st = kNeedExact;
-                    else total = cum[0][last];
+                const double bnd = (double)rule.topp * sum;
+                const int at = count_below(cum[0], br[0].n, bnd);
+                if (br[0].mass > bnd || at >= br[0].n) {
+                    st = kNeedSum64;  // not in this bracket
+                } else {
+                    kept = br[0].above + at + 1;
+                    total = cum[0][at];
                 }
             }
-            if (st == kDone) {
-                const int at = place(1, (double)rule.coin * total, 2.0 * err, st);
-                if (st == kDone && lane == 0)
-                    write_row(p, r, key_index(list[1][at]), key_value((uint32_t)(list[1][at] >> 32)), f.top,
-                              temperature, total, kept);
-            }
+            const double bnd = (double)rule.coin * total;
+            const int at = count_below(cum[1], br[1].n, bnd);
+            if (br[1].mass > bnd || at >= br[1].n) st = kNeedSum64;
+            if (st == kDone && lane == 0) write_row(p, r, list[1][at], f, total, kept);
             if (lane == 0) sm.status = st;
         }
         __syncthreads();
         const int st = sm.status;
+        if (st == kDone) return kDone;
+        limited_sum = sum;
         __syncthreads();
-        if (st != kNeedSum64) return st;
     }
     return kNeedExact;
 }
 
 // The first entry that equals the maximum.
 template <int NT, typename T>
-__device__ void take_first_max(const FilterLaunch& p, int r, const VecRow<T>& row, const RowFacts& f, FastSmem<NT>& sm) {
+__device__ __forceinline__ void take_first_max(const FilterLaunch& p, int r, const VecRow<T>& row, const RowFacts& f,
+                                               FastSmem<NT>& sm) {
     constexpr int E = VecRow<T>::E;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (threadIdx.x == 0) sm.first = 0x7FFFFFFF;
     __syncthreads();
-    for (int c = warp; c < f.chunks; c += NT / 32) {
+    for (int c = threadIdx.x; c < f.chunks; c += NT) {
         if (sm.chunk_max[c] != f.top) continue;
-        for (int s = c << f.chunk_shift; s < (c + 1) << f.chunk_shift; ++s) {
+        int at = 0x7FFFFFFF;
+        for (int j = 0; j < kU << f.chunk_shift; ++j) {
+            const int vec = ((((c >> 5) << f.chunk_shift) * kU + j) << 5) | (c & 31);
             float v[E];
-            row.load(s * 32 + lane, v);
-            int at = 0x7FFFFFFF;
+            VecRow<T>::widen(row.load(vec), v);
 #pragma unroll
-            for (int e = E - 1; e >= 0; --e)
-                if (v[e] == f.top) at = row.index(s * 32 + lane, e);
-            if (at != 0x7FFFFFFF) atomicMin(&sm.first, at);
+            for (int e = 0; e < E; ++e)
+                if (v[e] == f.top) at = min(at, row.index(vec, e));
         }
+        atomicMin(&sm.first, at);
     }
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -1128,24 +1285,36 @@ template <int NT, typename T>
 __global__ void __launch_bounds__(NT, 1024 / NT) filtered_sample_kernel(FilterLaunch p) {
     __shared__ FastSmem<NT> sm;
     const int r = blockIdx.x;
+    const VecRow<T> row(static_cast<const T*>(p.logits) + (long long)r * p.ld, p.vocab);
+    int shift = 0;
+    while (((row.batches - 1) >> shift) >= kChunkCap / 32) ++shift;
+    uint4 next[kU];  // on their way while the settings are read
+    if ((threadIdx.x >> 5) << shift < row.batches) row.load_batch((threadIdx.x >> 5) << shift, threadIdx.x & 31, next);
     RowRule rule = row_rule(p, r, threadIdx.x == 0);
-    if (threadIdx.x == 0) sm.coin = rule.coin;  // one thread draws, every thread decides by the same number
-    const T* x = static_cast<const T*>(p.logits) + (long long)r * p.ld;
-    const VecRow<T> row(x, p.vocab);
+    for (int i = threadIdx.x; i < kChunkBins; i += NT) sm.chunk_bin[i] = 0u;
+    if (threadIdx.x == 0) {
+        sm.coin = rule.coin;  // one thread draws, every thread decides by the same number
+        sm.hits = 0u;
+        sm.n[0] = 0u;
+    }
     RowFacts f;
-    f.z = rule.greedy ? 1.0f : kLog2e / rule.temperature;
-    int st = kNeedExact;
-    const bool plain = first_pass<NT>(row, sm, f);
+    f.z64 = rule.greedy ? 1.0 : 1.4426950408889634074 / (double)rule.temperature;
+    f.z = (float)f.z64;
+    const int k = rule.topk > 0 && rule.topk < p.vocab ? rule.topk : 0;
+    const bool open = !rule.greedy && k == 0 && !(rule.minp > 0.0f) && !(rule.topp > 0.0f && rule.topp < 1.0f);
+    if (open) first_pass<NT, T, true>(row, shift, next, sm, f);
+    else first_pass<NT, T, false>(row, shift, next, sm, f);
     rule.coin = sm.coin;
+    const bool plain = f.top > -__int_as_float(0x7F800000) && f.top < __int_as_float(0x7F800000);  // and no NaN
+    int st = kNeedExact;
     if (plain && rule.greedy) {
         take_first_max<NT>(p, r, row, f, sm);
         return;
     }
-    if (plain && f.sum > 0.0) {
+    if (plain && f.sum > 0.0f && f.sum < 1e30f) {
         f.minp_at = rule.minp > 0.0f
                         ? __double2float_ru((double)f.top + (double)rule.temperature * log(fmin((double)rule.minp, 1.0)))
                         : -__int_as_float(0x7F800000);
-        const int k = rule.topk > 0 && rule.topk < p.vocab ? rule.topk : 0;
         st = sample_from_list<NT>(p, r, row, rule, f, k, sm);
         if (st == kNeedBins) st = sample_by_bins<NT>(p, r, row, rule, f, k, sm);
     }
@@ -1154,20 +1323,19 @@ __global__ void __launch_bounds__(NT, 1024 / NT) filtered_sample_kernel(FilterLa
 }
 
 template <typename T>
-void launch_rows(const FilterLaunch& p, bool wide, cudaStream_t stream) {
-    if (wide) filtered_sample_kernel<1024, T><<<p.batch, 1024, 0, stream>>>(p);
+void launch_rows(const FilterLaunch& p, int num_sms, cudaStream_t stream) {
+    // Up to two rows an SM: all of an SM's threads on one row, for the row's
+    // latency.  More: several rows at a time on an SM, whose passes overlap.
+    if (p.batch <= 2 * num_sms) filtered_sample_kernel<1024, T><<<p.batch, 1024, 0, stream>>>(p);
     else filtered_sample_kernel<256, T><<<p.batch, 256, 0, stream>>>(p);
 }
 
 }  // namespace
 
 int launch_filtered_sample(const FilterLaunch& p, int num_sms, cudaStream_t stream) {
-    // Up to two rows an SM: all of an SM's threads on one row, for the row's
-    // latency.  More: four rows at a time on an SM, whose passes overlap.
-    const bool wide = p.batch <= 2 * num_sms;
-    if (p.dtype == kDtypeF32) launch_rows<float>(p, wide, stream);
-    else if (p.dtype == kDtypeBf16) launch_rows<__nv_bfloat16>(p, wide, stream);
-    else if (p.dtype == kDtypeF16) launch_rows<__half>(p, wide, stream);
+    if (p.dtype == kDtypeF32) launch_rows<float>(p, num_sms, stream);
+    else if (p.dtype == kDtypeBf16) launch_rows<__nv_bfloat16>(p, num_sms, stream);
+    else if (p.dtype == kDtypeF16) launch_rows<__half>(p, num_sms, stream);
     else return -(int)cudaErrorInvalidValue;
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? 1 : -(int)e;

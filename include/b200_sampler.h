@@ -340,7 +340,7 @@ int sampler_filtered(const SamplerFilterConfig* cfg, const void* logits, int bat
 /* x [rows, dim] (row r at x + r*ld, SAMPLER_DTYPE_*) as float8 e4m3 with one
  * fp32 scale per block of block_rows (1: activations, 128: weights) by 128
  * columns, the last blocks shorter where rows or dim end:
- *   s = max(amax / 448, 2^-126),  q = e4m3(x / s)   (nearest, ties to even)
+ *   s = max(amax / 448, 2^-126),  q = e4m3(x / s)   (nearest, ties to even, of the fp32 quotient)
  * A block holding a NaN or an infinity gets scale NaN and NaN values.
  *   out_q      [rows, dim] bytes, contiguous
  *   out_scales [ceil(rows / block_rows), ceil(dim / 128)] */

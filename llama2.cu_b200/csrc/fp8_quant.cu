@@ -6,170 +6,215 @@
 // Per block: amax = max |x|, s = max(RN(amax / 448), 2^-126), and
 // q = RN_e4m3(RN(x / s)) (448 is the largest e4m3 value; ties to even).  The
 // scale is rounded to fp32 before the division, so q * s is the nearest the
-// format has to x under the scale that is stored.  The clamp gives a block of
-// zeros a scale that can be divided by.  A block that holds a NaN or an
-// infinity gets scale NaN and NaN values: whatever is computed from it shows.
+// format has to x under the scale that is stored (a quotient within 2^-24 of a
+// tie counts as the tie).  The clamp gives a block of zeros a scale that can be
+// divided by.  A block that holds a NaN or an infinity gets scale NaN and NaN
+// values: whatever is computed from it shows.
 //
-// Both are bound by memory: an element is read once (4 or 2 bytes) and
-// written once (1 byte); the division is a product with the rounded
-// reciprocal and one FMA correction.
+// All three are bound by memory: an element is read once (4 or 2 bytes) and
+// written once (1 byte).  What stands in the way is the number of instructions
+// an element costs, so a lane has eight consecutive elements (the scale, its
+// reciprocal and the addresses are worked out once for eight), the division is
+// a product and two FMAs, and the kernels come in two forms: kWhole, where every
+// group of eight is whole and aligned, and one that checks each element.
 #include "device_common.cuh"
 #include "fp8_filter_kernels.cuh"
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
-#include <cuda_fp8.h>
 
 namespace b2s {
 namespace {
 
 constexpr int kQBlock = 128;
 constexpr int kQThreads = 256;
+constexpr int kN = 8;                // consecutive elements of a lane
+constexpr int kG = kQBlock / kN;     // lanes of a block's row: two rows a warp
 constexpr float kFp8Max = 448.0f;
 
 __device__ __forceinline__ float widen(float x) { return x; }
 __device__ __forceinline__ float widen(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float widen(__half x) { return __half2float(x); }
 
-// N consecutive elements from p (n of them exist, the rest read as 0).
-template <typename T, int N>
-__device__ __forceinline__ void load_elems(const T* p, int n, bool vec, float (&v)[N]) {
-    if (vec && n >= N) {
-        static_assert(sizeof(T) * N == 16, "16-byte loads");
-        const uint4 u = *reinterpret_cast<const uint4*>(p);
-        const T* t = reinterpret_cast<const T*>(&u);
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = widen(t[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = i < n ? widen(p[i]) : 0.0f;
-    }
-}
+// Eight elements as they are in memory.
+template <typename T>
+struct Raw {
+    uint32_t w[kN * sizeof(T) / 4];
+};
 
-template <int N>
-__device__ __forceinline__ void store_fp8(uint8_t* p, int n, bool vec, const float (&v)[N]) {
-    uint32_t w[N / 4];
+// Eight elements from p, of which n exist (kWhole: all of them, or none when n <= 0).
+template <typename T, bool kWhole>
+__device__ __forceinline__ Raw<T> load_raw(const T* p, int n) {
+    constexpr int W = kN * sizeof(T) / 4;
+    Raw<T> r;
 #pragma unroll
-    for (int i = 0; i < N / 4; ++i) {
-        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * i], v[4 * i + 1]), __NV_SATFINITE, __NV_E4M3);
-        const uint32_t hi =
-            __nv_cvt_float2_to_fp8x2(make_float2(v[4 * i + 2], v[4 * i + 3]), __NV_SATFINITE, __NV_E4M3);
-        w[i] = lo | (hi << 16);
-    }
-    if (vec && n >= N) {
-        if (N == 4) *reinterpret_cast<uint32_t*>(p) = w[0];
-        else *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[N / 4 - 1]);
-    } else {
+    for (int i = 0; i < W; ++i) r.w[i] = 0u;
+    if (kWhole) {
+        if (n > 0) {
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (i < n) p[i] = (uint8_t)(w[i / 4] >> (8 * (i & 3)));
-    }
-}
-
-// Largest magnitude as bits: NaN > infinity > every finite value.
-template <int N>
-__device__ __forceinline__ uint32_t abs_max_bits(const float (&v)[N]) {
-    uint32_t m = 0u;
-#pragma unroll
-    for (int i = 0; i < N; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-    return m;
-}
-
-__device__ __forceinline__ float block_scale(uint32_t amax_bits) {
-    if (amax_bits >= 0x7F800000u) return __uint_as_float(0x7FFFFFFFu);
-    return fmaxf(__fdiv_rn(__uint_as_float(amax_bits), kFp8Max), 0x1p-126f);
-}
-
-// v[i] / s, correctly rounded where the result matters to e4m3: the product
-// with r = RN(1/s) and one FMA correction (P. Markstein, "Computation of
-// elementary functions on the IBM RISC System/6000 processor", IBM J. Res.
-// Dev. 34(1), 1990).  With 2^-60 <= s <= 2^60 no intermediate of an x above
-// 2^-12 s leaves the normal range, and a smaller x gives 0 either way (half
-// the smallest e4m3 value is 2^-10).
-template <int N>
-__device__ __forceinline__ void divide_by_scale(float (&v)[N], float s) {
-    if (s >= 0x1p-60f && s <= 0x1p60f) {
-        const float r = __frcp_rn(s);
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const float q = __fmul_rn(v[i], r);
-            v[i] = __fmaf_rn(__fmaf_rn(-q, s, v[i]), r, q);
+            for (int i = 0; i < W / 4; ++i) {
+                const uint4 u = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+                r.w[4 * i] = u.x;
+                r.w[4 * i + 1] = u.y;
+                r.w[4 * i + 2] = u.z;
+                r.w[4 * i + 3] = u.w;
+            }
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = __fdiv_rn(v[i], s);
+        for (int i = 0; i < kN; ++i)
+            if (i < n) {
+                if (sizeof(T) == 4) r.w[i % W] = reinterpret_cast<const uint32_t*>(p)[i];
+                else r.w[i / 2] |= (uint32_t)reinterpret_cast<const unsigned short*>(p)[i] << (16 * (i & 1));
+            }
+    }
+    return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void widen_raw(const Raw<T>& r, float (&v)[kN]) {
+    const T* t = reinterpret_cast<const T*>(r.w);
+#pragma unroll
+    for (int i = 0; i < kN; ++i) v[i] = widen(t[i]);
+}
+
+// Two e4m3 values, a in the low byte: nearest, ties to even, up to 448, NaN kept.
+__device__ __forceinline__ uint32_t e4m3_pair(float a, float b) {
+    unsigned short r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(b), "f"(a));
+    return r;
+}
+
+template <bool kWhole>
+__device__ __forceinline__ void store_fp8(uint8_t* p, int n, const float (&v)[kN]) {
+    const uint32_t lo = e4m3_pair(v[0], v[1]) | (e4m3_pair(v[2], v[3]) << 16);
+    const uint32_t hi = e4m3_pair(v[4], v[5]) | (e4m3_pair(v[6], v[7]) << 16);
+    if (kWhole) {
+        if (n > 0) __stcs(reinterpret_cast<uint2*>(p), make_uint2(lo, hi));
+    } else {
+#pragma unroll
+        for (int i = 0; i < kN; ++i)
+            if (i < n) p[i] = (uint8_t)((i < 4 ? lo : hi) >> (8 * (i & 3)));
+    }
+}
+
+// Largest magnitude as bits (NaN > infinity > every finite value): of eight fp32
+// numbers, and of eight elements as they are in memory, where two 16-bit ones
+// are compared at once, accumulated into m and turned into fp32 bits at the end.
+__device__ __forceinline__ uint32_t abs_max_bits(const float (&v)[kN]) {
+    uint32_t m = 0u;
+#pragma unroll
+    for (int i = 0; i < kN; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+    return m;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t raw_abs_max(uint32_t m, const Raw<T>& r) {
+#pragma unroll
+    for (int i = 0; i < kN * (int)sizeof(T) / 4; ++i) {
+        if (sizeof(T) == 4) m = max(m, r.w[i] & 0x7FFFFFFFu);
+        else m = __vmaxu2(m, r.w[i] & 0x7FFF7FFFu);
+    }
+    return m;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t magnitude_bits(uint32_t m) {
+    if constexpr (sizeof(T) == 4) {
+        return m;
+    } else {
+        const unsigned short h = (unsigned short)max(m & 0xFFFFu, m >> 16);
+        return __float_as_uint(widen(*reinterpret_cast<const T*>(&h)));
+    }
+}
+// Largest of `m` in each half of the warp, the lanes of a block.
+__device__ __forceinline__ uint32_t half_warp_max(uint32_t m) {
+    const bool low = (threadIdx.x & 16) == 0;
+    const uint32_t a = __reduce_max_sync(kFullMask, low ? m : 0u), b = __reduce_max_sync(kFullMask, low ? 0u : m);
+    return low ? a : b;
+}
+
+// RN(amax / 448) by the reciprocal and one FMA correction, which is the correctly
+// rounded quotient while nothing leaves the normal range (P. Markstein,
+// "Computation of elementary functions on the IBM RISC System/6000 processor",
+// IBM J. Res. Dev. 34(1), 1990).
+__device__ __forceinline__ float block_scale(uint32_t amax_bits) {
+    if (amax_bits >= 0x7F800000u) return __uint_as_float(0x7FFFFFFFu);
+    const float a = __uint_as_float(amax_bits);
+    if (a < 0x1p-60f) return fmaxf(__fdiv_rn(a, kFp8Max), 0x1p-126f);
+    const float q = __fmul_rn(a, 1.0f / kFp8Max);
+    return __fmaf_rn(__fmaf_rn(-q, kFp8Max, a), 1.0f / kFp8Max, q);
+}
+
+// v[i] = RN(v[i] / s) in the same way.  With s in [2^-60, 2^60] no intermediate of
+// a v above 2^-12 s leaves the normal range, and a smaller v gives 0 either way
+// (half the smallest e4m3 value is 2^-10).
+__device__ __forceinline__ void divide_by_scale(float (&v)[kN], float s) {
+    if (s < 0x1p-60f || s > 0x1p60f) {  // both by the same power of two, into the range
+        const float f = s < 1.0f ? 0x1p80f : 0x1p-80f;
+        s *= f;
+#pragma unroll
+        for (int i = 0; i < kN; ++i) v[i] *= f;
+    }
+    const float r = __frcp_rn(s);
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+        const float q = __fmul_rn(v[i], r);
+        v[i] = __fmaf_rn(__fmaf_rn(-q, s, v[i]), r, q);
     }
 }
 
 // ---- activations: 1 x 128 blocks -------------------------------------------------
-// A block is one group of 128 / N lanes with 16 bytes of input each, so a warp
-// holds one fp32 block or two 16-bit ones; kUnits blocks a group are in flight.
-template <typename T>
+// A warp takes kUnits * 256 consecutive columns of a row at a time.
+template <typename T, bool kWhole>
 __global__ void __launch_bounds__(kQThreads)
-    quantize_rows_kernel(const T* x, long long ld, int rows, int dim, uint8_t* q, float* scales, int vec_in,
-                         int vec_out) {
-    constexpr int N = 16 / sizeof(T);
-    constexpr int G = kQBlock / N;  // lanes of a block
-    constexpr int kUnits = 4;
+    quantize_rows_kernel(const T* x, long long ld, unsigned items, unsigned segs, int dim, uint8_t* q, float* scales) {
+    constexpr int kUnits = sizeof(T) == 4 ? 2 : 4;
+    const int lane = threadIdx.x & 31;
     const int nb = (dim + kQBlock - 1) / kQBlock;
-    const long long units = (long long)rows * nb;
-    const int gl = threadIdx.x % G;
-    const long long groups = (long long)gridDim.x * (kQThreads / G);
-    const long long first = (long long)blockIdx.x * (kQThreads / G) + threadIdx.x / G;
-    for (long long u0 = first; u0 - first % (32 / G) < units; u0 += groups * kUnits) {  // whole warps stay together
-        float v[kUnits][N];
-        int n[kUnits], row[kUnits], blk[kUnits];
+    for (unsigned it = blockIdx.x * (kQThreads / 32) + (threadIdx.x >> 5); it < items; it += gridDim.x * (kQThreads / 32)) {
+        const unsigned row = it / segs;
+        const int col = (int)(it - row * segs) * (kUnits * 32 * kN) + lane * kN;
+        const T* xp = x + (long long)row * ld + col;
+        uint8_t* qp = q + (long long)row * dim + col;
+        Raw<T> raw[kUnits];
+#pragma unroll
+        for (int k = 0; k < kUnits; ++k)
+            raw[k] = load_raw<T, kWhole>(xp + k * 32 * kN, dim - col - k * 32 * kN);
 #pragma unroll
         for (int k = 0; k < kUnits; ++k) {
-            const long long u = u0 + k * groups;
-            row[k] = (int)(u / nb);
-            blk[k] = (int)(u - (long long)row[k] * nb);
-            n[k] = u < units ? min(N, dim - blk[k] * kQBlock - gl * N) : -1;
-            load_elems<T, N>(x + (n[k] > 0 ? (long long)row[k] * ld + blk[k] * kQBlock + gl * N : 0), n[k], vec_in != 0,
-                             v[k]);
-        }
-#pragma unroll
-        for (int k = 0; k < kUnits; ++k) {
-            uint32_t m = abs_max_bits(v[k]);
-#pragma unroll
-            for (int o = G / 2; o; o >>= 1) m = max(m, __shfl_xor_sync(kFullMask, m, o));
-            const float s = block_scale(m);
-            divide_by_scale(v[k], s);
-            if (u0 + k * groups < units && gl == 0) scales[(long long)row[k] * nb + blk[k]] = s;
-            if (n[k] > 0)
-                store_fp8<N>(q + (long long)row[k] * dim + blk[k] * kQBlock + gl * N, n[k], vec_out != 0, v[k]);
+            const int c = col + k * 32 * kN;
+            float v[kN];
+            widen_raw(raw[k], v);
+            const float s = block_scale(half_warp_max(magnitude_bits<T>(raw_abs_max(0u, raw[k]))));
+            divide_by_scale(v, s);
+            if (lane % kG == 0 && c < dim) scales[(long long)row * nb + c / kQBlock] = s;
+            store_fp8<kWhole>(qp + k * 32 * kN, dim - c, v);
         }
     }
 }
 
 // ---- weights: 128 x 128 blocks ----------------------------------------------------
-// One CTA a block, which it holds in registers (64 elements a thread) between
-// the maximum and the division.
-template <typename T>
-__global__ void __launch_bounds__(kQThreads)
-    quantize_blocks_kernel(const T* x, long long ld, int rows, int dim, uint8_t* q, float* scales, int vec_in,
-                           int vec_out) {
-    constexpr int N = 16 / sizeof(T);
-    constexpr int G = kQBlock / N;              // threads of a row
-    constexpr int kRowsPer = kQThreads / G;     // rows of one step
+// One CTA a block, which it holds in registers as it was loaded between the
+// maximum and the division.
+template <typename T, bool kWhole>
+__global__ void __launch_bounds__(kQThreads, sizeof(T) == 4 ? 2 : 4)
+    quantize_blocks_kernel(const T* x, long long ld, int rows, int dim, uint8_t* q, float* scales) {
+    constexpr int kRowsPer = kQThreads / kG;  // rows of one step
     constexpr int kSteps = kQBlock / kRowsPer;
     __shared__ uint32_t red[kQThreads / 32];
     const int nb = (dim + kQBlock - 1) / kQBlock;
-    const int br = blockIdx.x / nb, bc = blockIdx.x % nb;
-    const int col = bc * kQBlock + (threadIdx.x % G) * N;
-    const int row0 = br * kQBlock + threadIdx.x / G;
-    float v[kSteps][N];
+    const int br = blockIdx.x / nb, bc = blockIdx.x - br * nb;
+    const int col = bc * kQBlock + (threadIdx.x % kG) * kN;
+    const int row0 = br * kQBlock + threadIdx.x / kG;
+    const T* xp = x + (long long)row0 * ld + col;
+    uint8_t* qp = q + (long long)row0 * dim + col;
+    Raw<T> raw[kSteps];
     uint32_t m = 0u;
 #pragma unroll
-    for (int k = 0; k < kSteps; ++k) {
-        const int row = row0 + k * kRowsPer;
-        const int n = row < rows ? min(N, dim - col) : -1;
-        load_elems<T, N>(x + (n > 0 ? (long long)row * ld + col : 0), n, vec_in != 0, v[k]);
-    }
+    for (int k = 0; k < kSteps; ++k)
+        raw[k] = load_raw<T, kWhole>(xp + (long long)k * kRowsPer * ld, row0 + k * kRowsPer < rows ? dim - col : 0);
 #pragma unroll
-    for (int k = 0; k < kSteps; ++k) m = max(m, abs_max_bits(v[k]));
-#pragma unroll
-    for (int o = 16; o; o >>= 1) m = max(m, __shfl_xor_sync(kFullMask, m, o));
+    for (int k = 0; k < kSteps; ++k) m = raw_abs_max(m, raw[k]);
+    m = __reduce_max_sync(kFullMask, magnitude_bits<T>(m));
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
     __syncthreads();
 #pragma unroll
@@ -178,47 +223,43 @@ __global__ void __launch_bounds__(kQThreads)
     if (threadIdx.x == 0) scales[(long long)br * nb + bc] = s;
 #pragma unroll
     for (int k = 0; k < kSteps; ++k) {
-        const int row = row0 + k * kRowsPer;
-        const int n = row < rows ? min(N, dim - col) : -1;
-        divide_by_scale(v[k], s);
-        if (n > 0) store_fp8<N>(q + (long long)row * dim + col, n, vec_out != 0, v[k]);
+        float v[kN];
+        widen_raw(raw[k], v);
+        divide_by_scale(v, s);
+        store_fp8<kWhole>(qp + (long long)k * kRowsPer * dim, row0 + k * kRowsPer < rows ? dim - col : 0, v);
     }
 }
 
 // ---- RMSNorm and quantisation -----------------------------------------------------
 // v = weight * (x * r), r = 1 / sqrt(mean(x^2) + 1e-5), in fp32 as
 // rmsnorm_bf16_kernel forms it, then the 1 x 128 blocks of v.  One CTA a row;
-// the first kHeld groups of elements a thread meets stay in registers between
-// the sum and the division (every row up to 8192 wide in fp32, 16384 in 16
-// bits), the rest is read again.
-template <typename T>
-__global__ void __launch_bounds__(kQThreads)
-    rmsnorm_fp8_kernel(const T* x, long long ld, const float* weight, int dim, uint8_t* q, float* scales, int vec_in,
-                       int vec_out, int vec_w) {
-    constexpr int N = 16 / sizeof(T);
-    constexpr int G = kQBlock / N;
-    constexpr int kHeld = 8;
-    constexpr int kSpan = kQThreads * N;  // elements of one step of the CTA
+// the first kHeld groups of eight of a thread stay in registers between the sum
+// and the division (kHeld by the width, all of a row up to 8192 wide), the rest
+// is read again.
+template <typename T, int kHeld, bool kWhole>
+__global__ void __launch_bounds__(kQThreads, kHeld <= 2 ? 5 : 3)
+    rmsnorm_fp8_kernel(const T* x, long long ld, const float* weight, int dim, uint8_t* q, float* scales) {
+    constexpr int kSpan = kQThreads * kN;  // elements of one step of the CTA
     __shared__ float red[kQThreads / 32];
-    const T* xr = x + (long long)blockIdx.x * ld;
+    const int j0 = (int)threadIdx.x * kN;
+    const int warp_j0 = j0 - (int)(threadIdx.x & 31) * kN;
     const int nb = (dim + kQBlock - 1) / kQBlock;
-    float v[kHeld][N];
+    const T* xr = x + (long long)blockIdx.x * ld + j0;
+    uint8_t* qr = q + (long long)blockIdx.x * dim + j0;
+    float* sr = scales + (long long)blockIdx.x * nb;
+    Raw<T> raw[kHeld];
     float ss = 0.0f;
+    const auto add_squares = [&](const Raw<T>& r) {
+        float t[kN];
+        widen_raw(r, t);
 #pragma unroll
-    for (int k = 0; k < kHeld; ++k) {
-        const int j = k * kSpan + (int)threadIdx.x * N;
-        load_elems<T, N>(xr + (j < dim ? j : 0), dim - j, vec_in != 0, v[k]);
-    }
+        for (int i = 0; i < kN; ++i) ss = __fmaf_rn(t[i], t[i], ss);
+    };
 #pragma unroll
-    for (int k = 0; k < kHeld; ++k)
+    for (int k = 0; k < kHeld; ++k) raw[k] = load_raw<T, kWhole>(xr + k * kSpan, dim - j0 - k * kSpan);
 #pragma unroll
-        for (int i = 0; i < N; ++i) ss = __fmaf_rn(v[k][i], v[k][i], ss);
-    for (int j = kHeld * kSpan + (int)threadIdx.x * N; j < dim; j += kSpan) {
-        float t[N];
-        load_elems<T, N>(xr + j, dim - j, vec_in != 0, t);
-#pragma unroll
-        for (int i = 0; i < N; ++i) ss = __fmaf_rn(t[i], t[i], ss);
-    }
+    for (int k = 0; k < kHeld; ++k) add_squares(raw[k]);
+    for (int j = kHeld * kSpan; j0 + j < dim; j += kSpan) add_squares(load_raw<T, kWhole>(xr + j, dim - j0 - j));
 #pragma unroll
     for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(kFullMask, ss, o);
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = ss;
@@ -227,77 +268,76 @@ __global__ void __launch_bounds__(kQThreads)
 #pragma unroll
     for (int i = 0; i < kQThreads / 32; ++i) tot += red[i];
     const float r = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(tot, (float)dim), 1e-5f)));
-    uint8_t* qr = q + (long long)blockIdx.x * dim;
-    float* sr = scales + (long long)blockIdx.x * nb;
-    auto finish = [&](float (&t)[N], int j) {
-        float w[N];
-        if (vec_w && dim - j >= N) {
-#pragma unroll
-            for (int i = 0; i < N / 4; ++i) {
-                const float4 f = __ldg(reinterpret_cast<const float4*>(weight + j) + i);
-                w[4 * i] = f.x;
-                w[4 * i + 1] = f.y;
-                w[4 * i + 2] = f.z;
-                w[4 * i + 3] = f.w;
+    const auto finish = [&](const Raw<T>& raw8, int j) {
+        const int n = dim - j0 - j;  // elements that exist
+        float t[kN], w[kN];
+        widen_raw(raw8, t);
+        const float* wp = weight + j0 + j;
+        if (kWhole) {
+            float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f), b = a;
+            if (n > 0) {
+                a = __ldg(reinterpret_cast<const float4*>(wp));
+                b = __ldg(reinterpret_cast<const float4*>(wp) + 1);
             }
+            w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
+            w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
         } else {
 #pragma unroll
-            for (int i = 0; i < N; ++i) w[i] = j + i < dim ? __ldg(weight + j + i) : 0.0f;
+            for (int i = 0; i < kN; ++i) w[i] = i < n ? __ldg(wp + i) : 0.0f;
         }
 #pragma unroll
-        for (int i = 0; i < N; ++i) t[i] = __fmul_rn(w[i], __fmul_rn(r, t[i]));
-        if (j + N > dim) {  // a column past the row is 0 whatever r is
+        for (int i = 0; i < kN; ++i) t[i] = __fmul_rn(w[i], __fmul_rn(r, t[i]));
+        if (n < kN) {  // a column past the row is 0 whatever r is
 #pragma unroll
-            for (int i = 0; i < N; ++i)
-                if (j + i >= dim) t[i] = 0.0f;
+            for (int i = 0; i < kN; ++i)
+                if (i >= n) t[i] = 0.0f;
         }
-        uint32_t m = abs_max_bits(t);
-#pragma unroll
-        for (int o = G / 2; o; o >>= 1) m = max(m, __shfl_xor_sync(kFullMask, m, o));
-        const float s = block_scale(m);
+        const float s = block_scale(half_warp_max(abs_max_bits(t)));
         divide_by_scale(t, s);
-        if (j < dim) {
-            if (threadIdx.x % G == 0) sr[j / kQBlock] = s;
-            store_fp8<N>(qr + j, dim - j, vec_out != 0, t);
+        if (n > 0) {
+            if (threadIdx.x % kG == 0) sr[(j0 + j) / kQBlock] = s;
+            store_fp8<kWhole>(qr + j, n, t);
         }
     };
 #pragma unroll
-    for (int k = 0; k < kHeld; ++k) {
-        const int j = k * kSpan + (int)threadIdx.x * N;
-        if (j - (int)(threadIdx.x & 31) * N < dim) finish(v[k], j);  // whole warps: the shuffles need every lane
-    }
-    for (int j = kHeld * kSpan + (int)threadIdx.x * N; j - (int)(threadIdx.x & 31) * N < dim; j += kSpan) {
-        float t[N];
-        load_elems<T, N>(xr + (j < dim ? j : 0), dim - j, vec_in != 0, t);
-        finish(t, j);
-    }
+    for (int k = 0; k < kHeld; ++k)
+        if (warp_j0 + k * kSpan < dim) finish(raw[k], k * kSpan);  // whole warps: the maximum needs every lane
+    for (int j = kHeld * kSpan; warp_j0 + j < dim; j += kSpan) finish(load_raw<T, kWhole>(xr + j, dim - j0 - j), j);
 }
 
 bool aligned(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
-template <typename T>
+template <typename T, bool kWhole>
 cudaError_t launch_quantize_t(const QuantLaunch& p, int num_sms, cudaStream_t stream) {
-    constexpr int N = 16 / sizeof(T);
     const T* x = static_cast<const T*>(p.x);
     uint8_t* q = static_cast<uint8_t*>(p.q);
-    const int vec_in = aligned(x, 16) && p.ld % N == 0;
-    const int vec_out = aligned(q, N) && p.dim % N == 0;
-    const int nb = (p.dim + kQBlock - 1) / kQBlock;
     if (p.norm_weight) {
-        rmsnorm_fp8_kernel<T><<<p.rows, kQThreads, 0, stream>>>(x, p.ld, p.norm_weight, p.dim, q, p.scales, vec_in,
-                                                                vec_out, aligned(p.norm_weight, 16));
+        const auto launch = [&](auto kernel) {
+            kernel<<<p.rows, kQThreads, 0, stream>>>(x, p.ld, p.norm_weight, p.dim, q, p.scales);
+        };
+        constexpr int kSpan = kQThreads * kN;
+        if (p.dim <= kSpan) launch(rmsnorm_fp8_kernel<T, 1, kWhole>);
+        else if (p.dim <= 2 * kSpan) launch(rmsnorm_fp8_kernel<T, 2, kWhole>);
+        else launch(rmsnorm_fp8_kernel<T, 4, kWhole>);
     } else if (p.block_rows == 1) {
-        const long long units = (long long)p.rows * nb;
-        const long long per_cta = kQThreads / (kQBlock / N);
-        long long grid = (units + per_cta - 1) / per_cta;
-        if (grid > 8LL * num_sms) grid = 8LL * num_sms;
-        quantize_rows_kernel<T><<<(int)grid, kQThreads, 0, stream>>>(x, p.ld, p.rows, p.dim, q, p.scales, vec_in,
-                                                                     vec_out);
+        constexpr int kCols = (sizeof(T) == 4 ? 2 : 4) * 32 * kN;
+        const unsigned segs = (unsigned)(p.dim + kCols - 1) / kCols;
+        const unsigned items = (unsigned)p.rows * segs;
+        unsigned grid = (items + kQThreads / 32 - 1) / (kQThreads / 32);
+        if (grid > 16u * num_sms) grid = 16u * num_sms;
+        quantize_rows_kernel<T, kWhole><<<grid, kQThreads, 0, stream>>>(x, p.ld, items, segs, p.dim, q, p.scales);
     } else {
-        const int grid = ((p.rows + kQBlock - 1) / kQBlock) * nb;
-        quantize_blocks_kernel<T><<<grid, kQThreads, 0, stream>>>(x, p.ld, p.rows, p.dim, q, p.scales, vec_in, vec_out);
+        const int grid = ((p.rows + kQBlock - 1) / kQBlock) * ((p.dim + kQBlock - 1) / kQBlock);
+        quantize_blocks_kernel<T, kWhole><<<grid, kQThreads, 0, stream>>>(x, p.ld, p.rows, p.dim, q, p.scales);
     }
     return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t launch_quantize_t(const QuantLaunch& p, int num_sms, cudaStream_t stream) {
+    const bool whole = p.dim % kN == 0 && p.ld % (16 / (int)sizeof(T)) == 0 && aligned(p.x, 16) && aligned(p.q, 8) &&
+                       aligned(p.norm_weight, 16);
+    return whole ? launch_quantize_t<T, true>(p, num_sms, stream) : launch_quantize_t<T, false>(p, num_sms, stream);
 }
 
 }  // namespace

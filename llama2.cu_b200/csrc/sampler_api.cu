@@ -745,8 +745,8 @@ int quantize_call(const void* x, int x_dtype, const float* norm_weight, int rows
     if (((uintptr_t)x & (size - 1)) || ((uintptr_t)out_scales & 3u) || ((uintptr_t)norm_weight & 3u))
         return fail(SAMPLER_E_INVALID, "x, norm_weight or out_scales not aligned to its elements");
     const long long blocks = (((long long)rows + 127) / 128) * ((dim + 127) / 128);
-    if (block_rows == 128 && blocks > 0x7FFFFFFFLL)
-        return fail(SAMPLER_E_UNSUPPORTED, "%lld blocks in one call", blocks);
+    if ((block_rows == 128 ? blocks : (long long)rows * ((dim + 127) / 128)) > 0x3FFFFFFFLL)
+        return fail(SAMPLER_E_UNSUPPORTED, "rows %d by dim %d are too many blocks for one call", rows, dim);
     if (rows == 0) return SAMPLER_OK;
     DeviceCtx* c = nullptr;
     const int rc = get_ctx(&c);

@@ -317,69 +317,76 @@ def sample_batched_host(logits_np, temperature, topp, states_np, topp_rows_np=No
 
 
 # ---- filtered sampling and the 8-bit classifier ----
-_DTYPE_CODES = {}
+# These calls take microseconds on the device, so what they do on the host counts:
+# torch is looked up once, addresses go to ctypes as integers, and the current
+# device and stream are read without building objects for them.
+class _Torch:
+    """torch and what the calls below need of it, filled on first use."""
+    codes = {}
 
-
-def _dtype_code(t, what):
-    if not _DTYPE_CODES:
+    @classmethod
+    def load(cls):
         import torch
-        _DTYPE_CODES.update({torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16})
-    code = _DTYPE_CODES.get(t.dtype)
+        cls.torch, cls.empty, cls.f32, cls.i32, cls.i64 = torch, torch.empty, torch.float32, torch.int32, torch.int64
+        cls.f8, cls.u8 = torch.float8_e4m3fn, torch.uint8
+        cls.codes = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16}
+        cls.device = staticmethod(torch._C._cuda_getDevice)
+        cls.stream = staticmethod(torch._C._cuda_getCurrentRawStream)
+        return cls
+
+
+def _matrix(t, what):
+    """dtype code, rows, columns, row stride and device of a row-major CUDA matrix (any stride that keeps rows apart)."""
+    code = (_Torch.codes or _Torch.load().codes).get(t.dtype)
     if code is None:
         raise SamplerError(f"{what} must be float32, bfloat16 or float16, not {t.dtype}")
-    return code
+    if not t.is_cuda or t.dim() != 2:
+        raise SamplerError(f"{what} must be a CUDA matrix")
+    rows, cols = t.shape
+    ld, step = t.stride()
+    if cols > 1 and step != 1:
+        raise SamplerError(f"{what} must be row-major")
+    if rows <= 1:
+        ld = cols
+    elif ld < cols:
+        raise SamplerError(f"{what} has overlapping rows")
+    return code, rows, cols, ld, t.device
 
 
 def _vector(t, what, n, dtype, device):
     """Address of a contiguous vector of n elements on `device`; None passes."""
     if t is None:
         return None
-    if t.dtype != dtype or t.numel() != n or not t.is_contiguous() or t.device != device:
+    if t.dtype != dtype or t.numel() != n or t.device != device or not t.is_contiguous():
         raise SamplerError(f"{what} must be a contiguous {dtype} tensor of {n} elements on {device}")
     return t.data_ptr()
 
 
-def _matrix(t, what):
-    """Checks a row-major [R, C] CUDA tensor (any row stride that keeps rows apart)."""
-    if t.dim() != 2 or not t.is_cuda or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise SamplerError(f"{what} must be a row-major CUDA matrix")
-    if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
-        raise SamplerError(f"{what} has overlapping rows")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
-def _block_matrix(t, what, shape, dtype, device):
-    if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous() or t.device != device:
-        raise SamplerError(f"{what} must be a contiguous {dtype} tensor {list(shape)} on {device}")
+def _block_matrix(t, what, rows, cols, dtype, device):
+    """Address of a contiguous matrix of the given shape."""
+    if t.dtype != dtype or t.shape != (rows, cols) or t.device != device or not t.is_contiguous():
+        raise SamplerError(f"{what} must be a contiguous {dtype} tensor [{rows}, {cols}] on {device}")
     return t.data_ptr()
 
 
-def _on_device(device, rows, stream, fn, *args):
-    """fn(*args, stream) with the operands' device current, on `stream`
+def _on_device(device, rows, stream, name, *args):
+    """Calls entry point `name` with the operands' device current, on `stream`
     (default: that device's current one); nothing for an empty batch, whose
     tensors have no address."""
-    import torch
     if rows == 0:
         return
-    if torch.cuda.current_device() != device.index:
-        with torch.cuda.device(device):
-            return _on_device(device, rows, stream, fn, *args)
+    if _Torch.device() != device.index:
+        with _Torch.torch.cuda.device(device):
+            return _on_device(device, rows, stream, name, *args)
     if stream is None:
-        stream = torch.cuda.current_stream()
+        handle = _Torch.stream(device.index)
     elif stream.device != device:
         raise SamplerError(f"the stream is on {stream.device}, the operands on {device}")
-    rc = fn(*args, stream.cuda_stream)
+    else:
+        handle = stream.cuda_stream
+    rc = getattr(_lib or lib(), name)(*args, handle)
     if rc != 0:
-        _check(rc, fn.__name__)
-
-
-def _filter_rows(B, dev, temperature_rows, topk_rows, topp_rows, minp_rows, coins, rng_state):
-    import torch
-    f32 = torch.float32
-    return (_vector(temperature_rows, "temperature_rows", B, f32, dev),
-            _vector(topk_rows, "topk_rows", B, torch.int32, dev), _vector(topp_rows, "topp_rows", B, f32, dev),
-            _vector(minp_rows, "minp_rows", B, f32, dev), _vector(coins, "coins", B, f32, dev),
-            _vector(rng_state, "rng_state", B, torch.int64, dev))
+        _check(rc, name)
 
 
 def sample_filtered(logits, temperature, topk, topp, minp, rng_state=None, *, temperature_rows=None, topk_rows=None,
@@ -394,65 +401,64 @@ def sample_filtered(logits, temperature, topk, topp, minp, rng_state=None, *, te
     receive ln(p) of the id among the kept entries, their count, and the row's
     ROW_* bits.  Returns out_ids (int32 CUDA tensor [B]).  Asynchronous on
     `stream`."""
-    import torch
-    ld = _matrix(logits, "logits")
-    B, V = logits.shape
-    dev = logits.device
+    code, B, V, ld, dev = _matrix(logits, "logits")
+    f32, i32 = _Torch.f32, _Torch.i32
     if out_ids is None:
-        out_ids = torch.empty(B, dtype=torch.int32, device=dev)
-    i32 = torch.int32
-    cfg = SamplerFilterConfig(V, _dtype_code(logits, "logits"), temperature, topk, topp, minp)
-    _on_device(dev, B, stream, lib().sampler_filtered, ctypes.byref(cfg), logits.data_ptr(), B, ld,
-               *_filter_rows(B, dev, temperature_rows, topk_rows, topp_rows, minp_rows, coins, rng_state),
-               _vector(out_ids, "out_ids", B, i32, dev), _vector(logprobs_out, "logprobs_out", B, torch.float32, dev),
-               _vector(kept_out, "kept_out", B, i32, dev), _vector(row_flags, "row_flags", B, i32, dev))
+        out_ids = _Torch.empty(B, dtype=i32, device=dev)
+    cfg = SamplerFilterConfig(V, code, temperature, topk, topp, minp)
+    _on_device(dev, B, stream, "sampler_filtered", cfg, logits.data_ptr(), B, ld,
+               _vector(temperature_rows, "temperature_rows", B, f32, dev),
+               _vector(topk_rows, "topk_rows", B, i32, dev), _vector(topp_rows, "topp_rows", B, f32, dev),
+               _vector(minp_rows, "minp_rows", B, f32, dev), _vector(coins, "coins", B, f32, dev),
+               _vector(rng_state, "rng_state", B, _Torch.i64, dev), _vector(out_ids, "out_ids", B, i32, dev),
+               _vector(logprobs_out, "logprobs_out", B, f32, dev), _vector(kept_out, "kept_out", B, i32, dev),
+               _vector(row_flags, "row_flags", B, i32, dev))
     return out_ids
 
 
-def _fp8_outputs(x, block_rows, out, scales_out):
-    import torch
-    R, D = x.shape
-    shape = (-(-R // block_rows), -(-D // 128))
+def _fp8_outputs(R, D, block_rows, dev, out, scales_out):
+    rows, cols = -(-R // block_rows), (D + 127) // 128
     if out is None:
-        out = torch.empty(R, D, dtype=torch.float8_e4m3fn, device=x.device)
+        out = _Torch.empty((R, D), dtype=_Torch.f8, device=dev)
+        qp = out.data_ptr()
+    else:
+        qp = _block_matrix(out, "out", R, D, _Torch.f8, dev)
     if scales_out is None:
-        scales_out = torch.empty(shape, dtype=torch.float32, device=x.device)
-    return (out, scales_out, _block_matrix(out, "out", (R, D), torch.float8_e4m3fn, x.device),
-            _block_matrix(scales_out, "scales_out", shape, torch.float32, x.device))
+        scales_out = _Torch.empty((rows, cols), dtype=_Torch.f32, device=dev)
+        sp = scales_out.data_ptr()
+    else:
+        sp = _block_matrix(scales_out, "scales_out", rows, cols, _Torch.f32, dev)
+    return out, scales_out, qp, sp
 
 
 def quantize_fp8(x, block_rows=1, *, out=None, scales_out=None, stream=None):
     """x (float32, bfloat16 or float16 CUDA matrix [R, D], any row stride) as
     float8_e4m3fn [R, D] with one float32 scale per block of block_rows (1 for
     activations, 128 for weights) by 128 columns.  Returns (values, scales)."""
-    ld = _matrix(x, "x")
-    if block_rows not in (1, 128):
+    code, R, D, ld, dev = _matrix(x, "x")
+    if block_rows != 1 and block_rows != 128:
         raise SamplerError("block_rows must be 1 or 128")
-    out, scales_out, qp, sp = _fp8_outputs(x, block_rows, out, scales_out)
-    _on_device(x.device, x.shape[0], stream, lib().quantize_fp8, x.data_ptr(), _dtype_code(x, "x"), x.shape[0], x.shape[1], ld,
-               block_rows, qp, sp)
+    out, scales_out, qp, sp = _fp8_outputs(R, D, block_rows, dev, out, scales_out)
+    _on_device(dev, R, stream, "quantize_fp8", x.data_ptr(), code, R, D, ld, block_rows, qp, sp)
     return out, scales_out
 
 
 def rmsnorm_fp8(x, norm_weight, *, out=None, scales_out=None, stream=None):
     """quantize_fp8(norm_weight * x / rms(x)) with block_rows 1 in one pass: x
     float32, bfloat16 or float16 [B, D], norm_weight float32 [D]."""
-    import torch
-    ld = _matrix(x, "x")
-    out, scales_out, qp, sp = _fp8_outputs(x, 1, out, scales_out)
-    wp = _vector(norm_weight, "norm_weight", x.shape[1], torch.float32, x.device)
-    _on_device(x.device, x.shape[0], stream, lib().rmsnorm_fp8, x.data_ptr(), _dtype_code(x, "x"), wp, x.shape[0], x.shape[1], ld,
-               qp, sp)
+    code, B, D, ld, dev = _matrix(x, "x")
+    out, scales_out, qp, sp = _fp8_outputs(B, D, 1, dev, out, scales_out)
+    _on_device(dev, B, stream, "rmsnorm_fp8", x.data_ptr(), code,
+               _vector(norm_weight, "norm_weight", D, _Torch.f32, dev), B, D, ld, qp, sp)
     return out, scales_out
 
 
 def _fp8_weights(wcls, wcls_scales, D, dev):
-    import torch
     if wcls.dim() != 2 or wcls.shape[1] != D:
         raise SamplerError(f"wcls must be [V, {D}]")
     V = wcls.shape[0]
-    return (V, _block_matrix(wcls, "wcls", (V, D), torch.float8_e4m3fn, dev),
-            _block_matrix(wcls_scales, "wcls_scales", (-(-V // 128), -(-D // 128)), torch.float32, dev))
+    return (V, _block_matrix(wcls, "wcls", V, D, _Torch.f8, dev),
+            _block_matrix(wcls_scales, "wcls_scales", (V + 127) // 128, (D + 127) // 128, _Torch.f32, dev))
 
 
 def classifier_logits_fp8(hidden, hidden_scales, wcls, wcls_scales, logits_out=None, stream=None):
@@ -460,21 +466,21 @@ def classifier_logits_fp8(hidden, hidden_scales, wcls, wcls_scales, logits_out=N
     accumulation, from quantize_fp8's operands (hidden at block_rows 1 or
     rmsnorm_fp8's, wcls at 128).  logits_out: float32 (default) or bfloat16
     [B, V], any row stride."""
-    import torch
     if hidden.dim() != 2 or not hidden.is_cuda:
         raise SamplerError("hidden must be a CUDA matrix")
     B, D = hidden.shape
     dev = hidden.device
-    hp = _block_matrix(hidden, "hidden", (B, D), torch.float8_e4m3fn, dev)
-    hsp = _block_matrix(hidden_scales, "hidden_scales", (B, -(-D // 128)), torch.float32, dev)
+    if not _Torch.codes:
+        _Torch.load()
+    hp = _block_matrix(hidden, "hidden", B, D, _Torch.f8, dev)
+    hsp = _block_matrix(hidden_scales, "hidden_scales", B, (D + 127) // 128, _Torch.f32, dev)
     V, wp, wsp = _fp8_weights(wcls, wcls_scales, D, dev)
     if logits_out is None:
-        logits_out = torch.empty(B, V, dtype=torch.float32, device=dev)
-    ld = _matrix(logits_out, "logits_out")
-    if tuple(logits_out.shape) != (B, V) or logits_out.device != dev:
+        logits_out = _Torch.empty((B, V), dtype=_Torch.f32, device=dev)
+    code, rows, cols, ld, out_dev = _matrix(logits_out, "logits_out")
+    if rows != B or cols != V or out_dev != dev:
         raise SamplerError(f"logits_out must be [{B}, {V}] on {dev}")
-    _on_device(dev, B, stream, lib().classifier_logits_fp8, hp, hsp, wp, wsp, B, D, V, logits_out.data_ptr(),
-               _dtype_code(logits_out, "logits_out"), ld)
+    _on_device(dev, B, stream, "classifier_logits_fp8", hp, hsp, wp, wsp, B, D, V, logits_out.data_ptr(), code, ld)
     return logits_out
 
 
@@ -487,32 +493,33 @@ def classifier_fp8_sample_filtered(x, norm_weight, wcls, wcls_scales, temperatur
     is None), classifier_logits_fp8, sample_filtered.  logits_out: contiguous
     float32 or bfloat16 [B, V] that receives the logits (float32 otherwise).
     Returns out_ids."""
-    import torch
-    if x.dim() != 2 or not x.is_cuda or not x.is_contiguous():
-        raise SamplerError("x must be a contiguous CUDA matrix")
-    B, D = x.shape
-    dev = x.device
+    x_code, B, D, ld, dev = _matrix(x, "x")
+    if ld != D:
+        raise SamplerError("x must be contiguous")
     V, wp, wsp = _fp8_weights(wcls, wcls_scales, D, dev)
+    f32, i32 = _Torch.f32, _Torch.i32
     code, lp = DTYPE_F32, None
     if logits_out is not None:
-        code = _dtype_code(logits_out, "logits_out")
-        lp = _block_matrix(logits_out, "logits_out", (B, V), logits_out.dtype, dev)
-    L = lib()
-    n = L.classifier_fp8_workspace_bytes(B, D, V, code if lp is None else -1)
+        code = _Torch.codes.get(logits_out.dtype)
+        if code is None:
+            raise SamplerError("logits_out must be float32 or bfloat16")
+        lp = _block_matrix(logits_out, "logits_out", B, V, logits_out.dtype, dev)
+    n = lib().classifier_fp8_workspace_bytes(B, D, V, code if lp is None else -1)
     # from torch's allocator: ordered on the stream, and a graph's own inside a capture
-    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    ws = _Torch.empty(n, dtype=_Torch.u8, device=dev)
     if stream is not None:
         ws.record_stream(stream)
     if out_ids is None:
-        out_ids = torch.empty(B, dtype=torch.int32, device=dev)
-    i32 = torch.int32
+        out_ids = _Torch.empty(B, dtype=i32, device=dev)
     cfg = SamplerFilterConfig(V, code, temperature, topk, topp, minp)
-    _on_device(dev, B, stream, L.classifier_fp8_sample_filtered, ctypes.byref(cfg), x.data_ptr(), _dtype_code(x, "x"),
-               _vector(norm_weight, "norm_weight", D, torch.float32, dev), wp, wsp, B, D,
-               *_filter_rows(B, dev, temperature_rows, topk_rows, topp_rows, minp_rows, coins, rng_state),
-               _vector(out_ids, "out_ids", B, i32, dev), _vector(logprobs_out, "logprobs_out", B, torch.float32, dev),
-               _vector(kept_out, "kept_out", B, i32, dev), lp, _vector(row_flags, "row_flags", B, i32, dev),
-               ws.data_ptr(), n)
+    _on_device(dev, B, stream, "classifier_fp8_sample_filtered", cfg, x.data_ptr(), x_code,
+               _vector(norm_weight, "norm_weight", D, f32, dev), wp, wsp, B, D,
+               _vector(temperature_rows, "temperature_rows", B, f32, dev),
+               _vector(topk_rows, "topk_rows", B, i32, dev), _vector(topp_rows, "topp_rows", B, f32, dev),
+               _vector(minp_rows, "minp_rows", B, f32, dev), _vector(coins, "coins", B, f32, dev),
+               _vector(rng_state, "rng_state", B, _Torch.i64, dev), _vector(out_ids, "out_ids", B, i32, dev),
+               _vector(logprobs_out, "logprobs_out", B, f32, dev), _vector(kept_out, "kept_out", B, i32, dev), lp,
+               _vector(row_flags, "row_flags", B, i32, dev), ws.data_ptr(), n)
     return out_ids
 
 

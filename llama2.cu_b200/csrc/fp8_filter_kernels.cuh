@@ -37,6 +37,8 @@ struct Fp8GemmLaunch {
     int out_bf16;
     long long ld;
     int* error_word;
+    int tile_rows;          // set by the launch: rows of the operand on the TMEM lanes in a tile
+    int vec_out;            // set by the launch: rows of logits start on 16-byte boundaries
 };
 constexpr int kFp8MaxSmem = 227 * 1024;
 

@@ -37,10 +37,9 @@ struct Fp8GemmLaunch {
     int out_bf16;
     long long ld;
     int* error_word;
-    int tile_rows;          // set by the launch: rows of the operand on the TMEM lanes in a tile
+    int box_rows;           // set by the launch: rows of H that a tile loads
     int vec_out;            // set by the launch: rows of logits start on 16-byte boundaries
 };
-constexpr int kFp8MaxSmem = 227 * 1024;
 
 // Sampling by temperature, top-k, top-p and min-p (filtered_sample.cu).
 struct FilterLaunch {

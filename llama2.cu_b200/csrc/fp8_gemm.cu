@@ -10,20 +10,22 @@
 // (two per instruction, fma.f32x2) while the tensor core works on the next block
 // in the other buffer.  One persistent CTA per SM:
 //   warp 0      TMA producer: operand boxes of 128 bytes by the tile's rows,
-//               128-byte swizzle, into a ring of stages
+//               128-byte swizzle, into a ring of four stages
 //   warp 1      MMA issuer (one thread)
 //   warp 2      TMEM allocation / release
-//   warps 4..   fold: one TMEM lane a thread, 128 columns at most; at the end
-//               of a tile they write the logits
-// Large batches have H on the 128 TMEM lanes (its scale is the thread's own, W's
-// one number per block: one FMA an element) and 256 columns of W, which two
-// warpgroups fold; a thread then holds 128 sums, so the fold warps take registers
-// over from the others (setmaxnreg).  They write through shared memory, 32 x 32
-// logits a warp at a time, so that whole 128-byte lines go out.
-// Small batches (kWLanes) have W on the lanes: NT is the padded batch, H's scales
-// come from shared memory, and reading W is all that counts.  The rows of W are
-// cut into tiles of equal height, at most 128, such that every SM gets the same
-// number (32000 rows: 294 tiles of 109, two an SM, not 250 of 128).
+//   warps 4-11  fold: one row of H a thread, 128 columns (rows of W) a warpgroup;
+//               at the end of a tile they write the logits
+// H is on the 128 TMEM lanes whatever the batch is: an instruction costs its 128
+// lanes' time anyway (about 97 ns with 16 columns, 130 with 256), so W on the
+// lanes, which looks better for a single row, was slower there too (35 us for
+// 1 x 4096 x 32000).  A tile has up to 256 columns, in 32s, chosen by the host so that
+// the tiles fill the SMs evenly.  A fold thread holds 128 sums, so the fold warps
+// take registers over from the others (setmaxnreg).  They write through shared
+// memory, 32 x 32 logits a warp at a time, so that whole 128-byte lines go out.
+//
+// What bounds it: for large batches the way of a TMEM buffer from its last product
+// to its next first one (commit, loads, release, issue: some 650 ns, of which the
+// other buffer's product covers 520), for small ones the stream of W.
 // Every mbarrier wait is bounded; a timeout sets the error word and drains
 // the pipeline.
 #include "device_common.cuh"
@@ -40,59 +42,45 @@
 namespace b2s {
 namespace {
 
-constexpr int kFM = 128;      // TMEM lanes of a tile
+constexpr int kFM = 128;      // rows of H in a tile (TMEM lanes)
+constexpr int kFN = 256;      // columns of a tile, at most; the stride of the TMEM buffers
 constexpr int kFK = 128;      // K of a block, a stage and one accumulation
+constexpr int kFStages = 4;
+constexpr int kFCols = kFN / 2;                 // columns a warpgroup folds
+constexpr int kFThreads = 128 + 2 * 128;
 constexpr int kFABytes = kFM * kFK;
+constexpr int kFBBytes = kFN * kFK;
+constexpr int kFTmemCols = 2 * kFN;
 constexpr int kFGroupM = 16;  // row tiles swept together (L2 reuse of W)
 
-template <int NT, bool kWLanes>
-struct Fp8Cfg {
-    static constexpr int kGroups = NT > 128 ? NT / 128 : 1;  // warpgroups of the fold
-    static constexpr int kCols = NT / kGroups;               // columns a thread folds
-    static constexpr int kThreads = 128 + 128 * kGroups;
-    static constexpr int kBBytes = NT * kFK;
-    static constexpr int kStages = (NT == 256) ? 4 : (NT >= 64 ? 6 : 8);
-    static constexpr bool kStaged = !kWLanes;                // logits leave through shared memory
-    static constexpr int kStageOut = kStaged ? 4 * kGroups * 32 * 32 : 1;
-    static constexpr int kTmemCols = 2 * NT < 32 ? 32 : 2 * NT;
-    // Instruction descriptor, kind::f8f6f4: fp32 accumulator (bits 4-5 = 1), A and B e4m3 (bits 7-9,
-    // 10-12 = 0), both K-major (bits 15, 16 = 0), N >> 3 in bits 17-22, M >> 4 in bits 24-28.
-    static constexpr uint32_t kIdesc = (1u << 4) | ((uint32_t)(NT >> 3) << 17) | ((uint32_t)(kFM >> 4) << 24);
-};
-
-template <int kStages>
-struct Fp8Bars {
-    unsigned long long full[kStages];
-    unsigned long long empty[kStages];
+struct Fp8Smem {
+    uint8_t a[kFStages][kFABytes];  // 1024-byte aligned (the swizzle atom)
+    uint8_t b[kFStages][kFBBytes];
+    float out[8][32 * 32];          // by fold warp
+    unsigned long long full[kFStages];
+    unsigned long long empty[kFStages];
     unsigned long long tmem_full[2];
     unsigned long long tmem_empty[2];
     unsigned long long drain;
     uint32_t tmem_base;
     int abort;
 };
-
-template <int NT, bool kWLanes>
-struct Fp8Smem {
-    using C = Fp8Cfg<NT, kWLanes>;
-    uint8_t a[C::kStages][kFABytes];  // 1024-byte aligned (the swizzle atom)
-    uint8_t b[C::kStages][C::kBBytes];
-    float out[C::kStageOut];
-    Fp8Bars<C::kStages> bar;
-};
+constexpr size_t kFp8SmemBytes = sizeof(Fp8Smem) + 1024;  // + alignment slack
+static_assert(kFp8SmemBytes <= 227 * 1024, "one CTA's shared memory");
 
 // D[tmem] (+)= A[smem] . B[smem]^T, kind::f8f6f4 (e4m3 inputs, fp32 accumulator)
 __device__ __forceinline__ void tc_mma_fp8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
-                                           uint32_t accumulate) {
+                                           bool accumulate) {
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"((uint32_t)accumulate)
         : "memory");
 }
 
-// 32 (16) consecutive fp32 columns of this thread's TMEM lane; the values are
-// there after tmem_wait on them.
+// 32 consecutive fp32 columns of this thread's TMEM lane; the values are there
+// after tmem_wait on them.
 __device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[32]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
@@ -103,23 +91,8 @@ __device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[32]) {
           "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(taddr));
 }
-__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
-        "%14, %15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr));
-}
 // Waits for this thread's TMEM loads; the values pass through, so that no use of
 // them can be moved before it.
-__device__ __forceinline__ void tmem_wait(uint32_t (&r)[16]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
-                 :
-                 : "memory");
-}
 __device__ __forceinline__ void tmem_wait(uint32_t (&r)[32]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
                  : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
@@ -148,272 +121,293 @@ __device__ __forceinline__ float2 halves_of(unsigned long long v) {
     return f;
 }
 
-template <class Bars>
-__device__ __forceinline__ bool fp8_aborted(const Bars& b) {
-    return *(const volatile int*)&b.abort != 0;
-}
-template <class Bars>
-__device__ __forceinline__ bool fp8_wait(unsigned long long* bar, unsigned parity, Bars& b, int* error_word) {
-    if (mbar_wait_bounded(bar, parity)) return true;
-    b.abort = 1;
+__device__ __forceinline__ bool fp8_aborted(const Fp8Smem& sm) { return *(const volatile int*)&sm.abort != 0; }
+// Bounded wait, inline: one thread issues all products and one all copies, and
+// every instruction of their loops is on a block's way.
+__device__ __forceinline__ bool fp8_wait(unsigned long long* bar, unsigned parity, Fp8Smem& sm, int* error_word) {
+    for (unsigned i = 0; i < kSpinLimit; ++i)
+        if (mbar_try_wait(bar, parity)) return true;
+    sm.abort = 1;
     atomicOr(error_word, 2);
     return false;
 }
 
-__device__ __forceinline__ void store_logit(const Fp8GemmLaunch& p, long long at, float v) {
-    if (p.out_bf16) static_cast<__nv_bfloat16*>(p.logits)[at] = __float2bfloat16_rn(v);
-    else static_cast<float*>(p.logits)[at] = v;
-}
-
-// 32 x 32 logits from the warp's shared memory: rows row0 .., columns col0 ...
-// Whole 16-byte pieces where the rows allow it, else 32 columns of a row at a time.
-__device__ __forceinline__ void write_block(const Fp8GemmLaunch& p, const float* out, int row0, int col0, int lane) {
-    const float4* out4 = reinterpret_cast<const float4*>(out);
-    if (p.vec_out && col0 + 32 <= p.vocab) {
-        if (p.out_bf16) {
+// A warp's 32 rows of `out`, 128 bytes each (32 fp32 or 64 bf16 logits, the 16-byte
+// piece j of row r at piece j ^ (r % 8)), to rows row0 .. and the n columns from
+// col0 on.  Whole 16-byte pieces where the rows allow it; else a row at a time, bf16
+// in pairs that start on 4 bytes.
+template <typename T>
+__device__ __forceinline__ void write_block(const Fp8GemmLaunch& p, const T* out, int row0, int col0, int n, int lane) {
+    constexpr int kPer = 16 / sizeof(T);  // elements of a piece
+    const uint4* out4 = reinterpret_cast<const uint4*>(out);
+    T* const to = static_cast<T*>(p.logits) + (long long)row0 * p.ld + col0;
+    const int rows = min(32, p.batch - row0);
+    const auto at = [&](int r, int c) { return out[r * 8 * kPer + (((c / kPer) ^ (r & 7)) * kPer) + c % kPer]; };
+    if (p.vec_out && n % kPer == 0) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int r = i * 8 + lane / 4, j = 2 * (lane & 3);
-                const float4 a = out4[r * 8 + (j ^ (r & 7))], b = out4[r * 8 + ((j + 1) ^ (r & 7))];
-                const __nv_bfloat162 w[4] = {__floats2bfloat162_rn(a.x, a.y), __floats2bfloat162_rn(a.z, a.w),
-                                             __floats2bfloat162_rn(b.x, b.y), __floats2bfloat162_rn(b.z, b.w)};
-                if (row0 + r < p.batch)
-                    *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.logits) + (long long)(row0 + r) * p.ld + col0 +
-                                              8 * (lane & 3)) = *reinterpret_cast<const uint4*>(w);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int r = i * 4 + lane / 8, j = lane & 7;
-                const float4 a = out4[r * 8 + (j ^ (r & 7))];
-                if (row0 + r < p.batch)
-                    *reinterpret_cast<float4*>(static_cast<float*>(p.logits) + (long long)(row0 + r) * p.ld + col0 + 4 * j) = a;
-            }
+        for (int i = 0; i < 8; ++i) {
+            const int r = i * 4 + lane / 8, j = lane & 7;
+            if (r < rows && j * kPer < n) *reinterpret_cast<uint4*>(to + r * p.ld + j * kPer) = out4[r * 8 + (j ^ (r & 7))];
         }
-    } else if (col0 + lane < p.vocab) {
+    } else if (sizeof(T) == 4) {
 #pragma unroll 4
         for (int r = 0; r < 32; ++r)
-            if (row0 + r < p.batch)
-                store_logit(p, (long long)(row0 + r) * p.ld + col0 + lane, out[r * 32 + (((lane / 4) ^ (r & 7)) << 2) + (lane & 3)]);
+            if (r < rows && lane < n) to[r * p.ld + lane] = at(r, lane);
+    } else {
+#pragma unroll 4
+        for (int r = 0; r < 32; ++r) {
+            if (r >= rows) break;
+            T* const q = to + r * p.ld;
+            const int odd = (int)(reinterpret_cast<uintptr_t>(q) >> 1 & 1u), c = 2 * lane + odd;
+            if (c + 1 < n) {
+                T pair[2] = {at(r, c), at(r, c + 1)};
+                *reinterpret_cast<uint32_t*>(q + c) = *reinterpret_cast<const uint32_t*>(pair);
+            } else if (c < n) {
+                q[c] = at(r, c);
+            }
+            if (odd && lane == 0) q[0] = at(r, 0);
+        }
     }
 }
 
-template <int NT, bool kWLanes>
-__global__ void __launch_bounds__(Fp8Cfg<NT, kWLanes>::kThreads, 1)
-    fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
+__device__ __forceinline__ void fp8_tile_coords(int tile, int mt, int nt, int& m_blk, int& n_blk) {
+    const int per_group = kFGroupM * nt;
+    const int g = tile / per_group;
+    const int r = tile - g * per_group;
+    const int gm = min(kFGroupM, mt - g * kFGroupM);
+    n_blk = r / gm;
+    m_blk = g * kFGroupM + (r - n_blk * gm);
+}
+
+// The fold warps' part: 128 columns of every tile of NC.  Both warpgroups run the
+// same instructions, also where NC leaves the second fewer columns (it folds what
+// its TMEM columns hold and writes NC - 128): a loop of its own for it cost a
+// quarter of the rate, in instruction fetches.
+template <int NC>
+__device__ __forceinline__ void fold_tiles(const Fp8GemmLaunch& p, Fp8Smem& sm, uint32_t tmem, int mt, int nt, int nk) {
+    constexpr bool kAligned = NC % kFK == 0;  // the columns lie in one block of 128 rows of W
+    constexpr int kCols = kFCols;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q = warp & 3;
+    const int col0 = warp < 8 ? 0 : kFCols;
+    const int ntiles = mt * nt;
+    const int wblocks = (p.vocab + kFK - 1) / kFK;
+    unsigned it = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; tile < ntiles && ok; tile += gridDim.x) {
+        int mb, nb;
+        fp8_tile_coords(tile, mt, nt, mb, nb);
+        const int row0 = mb * kFM + q * 32, row = row0 + lane;
+        const int wcol = nb * NC + col0;
+        if (NC < kFN && row0 >= p.batch) {  // no rows of H here: the buffers are given back unread
+            for (int k = 0; k < nk; ++k, ++it) {
+                ok = ok && fp8_wait(&sm.tmem_full[it & 1u], it >> 1 & 1u, sm, p.error_word);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.tmem_empty[it & 1u]);
+            }
+            ok = __all_sync(kFullMask, ok ? 1 : 0);
+            continue;
+        }
+        unsigned long long acc[kCols / 2];
+#pragma unroll
+        for (int j = 0; j < kCols / 2; ++j) acc[j] = 0ull;
+        // `bound` of the columns belong to the first of the two blocks of W that they can lie in
+        const int wb = wcol / kFK, bound = (wb + 1) * kFK - wcol;
+        const float* own_scale = p.h_scales + (long long)row * nk;
+        const float* lo_scale = p.w_scales + (long long)wb * nk;
+        // The scales are on their way for two blocks before they are multiplied: L1, beside
+        // 227 KB of shared memory, does not hold the rows' lines from block to block.
+        const bool use = row < p.batch && wb < wblocks, use_hi = !kAligned && use && bound < kCols && wb + 1 < wblocks;
+        float own0 = use ? __ldg(own_scale) : 0.0f, own1 = use && nk > 1 ? __ldg(own_scale + 1) : 0.0f;
+        float lo0 = use ? __ldg(lo_scale) : 0.0f, lo1 = use && nk > 1 ? __ldg(lo_scale + 1) : 0.0f;
+        float hi0 = use_hi ? __ldg(lo_scale + nk) : 0.0f, hi1 = use_hi && nk > 1 ? __ldg(lo_scale + nk + 1) : 0.0f;
+        for (int k = 0; k < nk; ++k, ++it) {
+            const unsigned buf = it & 1u;
+            const bool more = k + 2 < nk;
+            const float own2 = use && more ? __ldg(own_scale + k + 2) : 0.0f;
+            const float lo2 = use && more ? __ldg(lo_scale + k + 2) : 0.0f;
+            const float hi2 = use_hi && more ? __ldg(lo_scale + nk + k + 2) : 0.0f;
+            // After a wait that ran out the rest of the tile is folded without waiting (and not
+            // written): nothing but the wait stands between a buffer's arrival and its loads (a
+            // look at the abort word here cost a quarter of the rate).
+            ok = ok && fp8_wait(&sm.tmem_full[buf], it >> 1 & 1u, sm, p.error_word);
+            __syncwarp();
+            tc_fence_after();
+            const uint32_t src = tmem + ((uint32_t)(q * 32) << 16) + buf * kFN + (uint32_t)col0;
+            const unsigned long long s_lo = pair_of(own0 * lo0, own0 * lo0);
+            const unsigned long long s_hi = kAligned ? s_lo : pair_of(own0 * hi0, own0 * hi0);
+#pragma unroll
+            for (int c = 0; c < kCols; c += 64) {
+                uint32_t t0[32], t1[32];
+                tmem_load(src + (uint32_t)c, t0);
+                tmem_load(src + (uint32_t)(c + 32), t1);
+                tmem_wait(t0);
+                tmem_wait(t1);
+                if (c + 64 >= kCols) {  // the buffer has been read
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sm.tmem_empty[buf]);
+                }
+                const unsigned long long f0 = kAligned || c < bound ? s_lo : s_hi;
+                const unsigned long long f1 = kAligned || c + 32 < bound ? s_lo : s_hi;
+#pragma unroll
+                for (int j = 0; j < 32; j += 2) fold2(acc[(c + j) / 2], t0[j], t0[j + 1], f0);
+#pragma unroll
+                for (int j = 0; j < 32; j += 2) fold2(acc[(c + 32 + j) / 2], t1[j], t1[j + 1], f1);
+            }
+            own0 = own1, own1 = own2;
+            lo0 = lo1, lo1 = lo2;
+            hi0 = hi1, hi1 = hi2;
+        }
+        ok = __all_sync(kFullMask, ok ? 1 : 0);
+        if (!ok) break;
+        // 128 bytes of each row at a time through the warp's shared memory, so that whole lines go
+        // out; piece j of row r is at piece j ^ (r % 8), so neither side meets bank conflicts
+        const int left = min(NC - col0, p.vocab - wcol);  // columns to write
+        uint4* const out4 = reinterpret_cast<uint4*>(sm.out[warp - 4]);
+        if (p.out_bf16) {
+#pragma unroll
+            for (int c = 0; c < kCols; c += 64) {
+                if (c >= left) break;
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 a = halves_of(acc[c / 2 + 4 * j + i]);
+                        const __nv_bfloat162 h = __floats2bfloat162_rn(a.x, a.y);
+                        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+                    }
+                    out4[lane * 8 + (j ^ (lane & 7))] = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+                __syncwarp();
+                write_block(p, reinterpret_cast<const __nv_bfloat16*>(out4), row0, wcol + c, min(64, left - c), lane);
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < kCols; c += 32) {
+                if (c >= left) break;
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float2 a = halves_of(acc[c / 2 + 2 * j]), b = halves_of(acc[c / 2 + 2 * j + 1]);
+                    out4[lane * 8 + (j ^ (lane & 7))] = make_uint4(__float_as_uint(a.x), __float_as_uint(a.y),
+                                                                   __float_as_uint(b.x), __float_as_uint(b.y));
+                }
+                __syncwarp();
+                write_block(p, reinterpret_cast<const float*>(out4), row0, wcol + c, min(32, left - c), lane);
+            }
+        }
+    }
+}
+
+template <int NC>
+__global__ void __launch_bounds__(kFThreads, 1)
+    fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_h, const __grid_constant__ CUtensorMap tmap_w,
                     Fp8GemmLaunch p) {
-    using C = Fp8Cfg<NT, kWLanes>;
     extern __shared__ __align__(16) unsigned char fsm_raw[];
-    Fp8Smem<NT, kWLanes>& sm =
-        *reinterpret_cast<Fp8Smem<NT, kWLanes>*>((reinterpret_cast<uintptr_t>(fsm_raw) + 1023) & ~(uintptr_t)1023);
-    auto& bar = sm.bar;
+    Fp8Smem& sm = *reinterpret_cast<Fp8Smem*>((reinterpret_cast<uintptr_t>(fsm_raw) + 1023) & ~(uintptr_t)1023);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int rows_a = kWLanes ? p.vocab : p.batch, rows_b = kWLanes ? p.batch : p.vocab;
-    const int mt = (rows_a + p.tile_rows - 1) / p.tile_rows;  // tile_rows: 128, or fewer rows of W
-    const int nt = (rows_b + NT - 1) / NT;
+    const int mt = (p.batch + kFM - 1) / kFM;
+    const int nt = (p.vocab + NC - 1) / NC;
     const int ntiles = mt * nt;
     const int nk = (p.dim + kFK - 1) / kFK;
 
     if (tid == 0) {
-        for (int s = 0; s < C::kStages; ++s) {
-            mbar_init(&bar.full[s], 1);
-            mbar_init(&bar.empty[s], 1);
+        for (int s = 0; s < kFStages; ++s) {
+            mbar_init(&sm.full[s], 1);
+            mbar_init(&sm.empty[s], 1);
         }
         for (int a = 0; a < 2; ++a) {
-            mbar_init(&bar.tmem_full[a], 1);
-            mbar_init(&bar.tmem_empty[a], 4 * C::kGroups);  // one arrival per fold warp
+            mbar_init(&sm.tmem_full[a], 1);
+            mbar_init(&sm.tmem_empty[a], NC > kFCols ? 8 : 4);  // one arrival per fold warp
         }
-        mbar_init(&bar.drain, 1);
-        bar.abort = 0;
+        mbar_init(&sm.drain, 1);
+        sm.abort = 0;
         fence_mbar_init();
     }
     if (warp == 2) {
-        tmem_alloc(smem_addr(&bar.tmem_base), C::kTmemCols);
+        tmem_alloc(smem_addr(&sm.tmem_base), kFTmemCols);
         tmem_relinquish();
-    }
-    // small batches: H's scales, transposed to [block][row], behind the ring
-    float* hs_sm = reinterpret_cast<float*>(&sm + 1);
-    if (kWLanes) {
-        for (int i = tid; i < nk * NT; i += C::kThreads) {
-            const int b = i % NT, g = i / NT;
-            hs_sm[i] = b < p.batch ? p.h_scales[(long long)b * nk + g] : 0.0f;
-        }
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = bar.tmem_base;
+    const uint32_t tmem = sm.tmem_base;
 
-    auto coords = [&](int tile, int& mb, int& nb) {
-        const int per_group = kFGroupM * nt;
-        const int g = tile / per_group;
-        const int r = tile - g * per_group;
-        const int gm = min(kFGroupM, mt - g * kFGroupM);
-        nb = r / gm;
-        mb = g * kFGroupM + (r - nb * gm);
-    };
-
-    // 384 threads at 168 registers: the two fold warpgroups take 208, the other 88
+    // 384 threads at 168 registers: the two fold warpgroups take 216, the other 72
     if (warp < 4) {
-    if (C::kGroups == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    if (warp == 0 && lane == 0) {
-        // ---- TMA producer
-        int stage = 0;
-        unsigned phase = 0;
-        for (int tile = blockIdx.x; tile < ntiles && !fp8_aborted(bar); tile += gridDim.x) {
-            int mb, nb;
-            coords(tile, mb, nb);
-            for (int k = 0; k < nk; ++k) {
-                if (!fp8_wait(&bar.empty[stage], phase ^ 1u, bar, p.error_word)) break;
-                mbar_arrive_expect_tx(&bar.full[stage], p.tile_rows * kFK + C::kBBytes);
-                tma_load_2d(sm.a[stage], &tmap_a, k * kFK, mb * p.tile_rows, &bar.full[stage]);
-                tma_load_2d(sm.b[stage], &tmap_b, k * kFK, nb * NT, &bar.full[stage]);
-                if (++stage == C::kStages) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (warp == 0 && lane == 0) {
+            // ---- TMA producer
+            const unsigned bytes = (unsigned)(p.box_rows + NC) * kFK;
+            unsigned stage = 0, phase = 0;
+            for (int tile = blockIdx.x; tile < ntiles && !fp8_aborted(sm); tile += gridDim.x) {
+                int mb, nb;
+                fp8_tile_coords(tile, mt, nt, mb, nb);
+                for (int k = 0; k < nk; ++k) {
+                    if (!fp8_wait(&sm.empty[stage], phase ^ 1u, sm, p.error_word)) break;
+                    mbar_arrive_expect_tx(&sm.full[stage], bytes);
+                    tma_load_2d(sm.a[stage], &tmap_h, k * kFK, mb * kFM, &sm.full[stage]);
+                    tma_load_2d(sm.b[stage], &tmap_w, k * kFK, nb * NC, &sm.full[stage]);
+                    if (++stage == kFStages) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+            }
+            // drain: every stage this thread filled completes before the CTA exits
+            for (int s = 0; s < kFStages; ++s) {
+                if (!mbar_wait_bounded(&sm.empty[stage], phase ^ 1u)) break;
+                if (++stage == kFStages) {
                     stage = 0;
                     phase ^= 1u;
                 }
             }
-        }
-        // drain: every stage this thread filled completes before the CTA exits
-        for (int s = 0; s < C::kStages; ++s) {
-            if (!mbar_wait_bounded(&bar.empty[stage], phase ^ 1u)) break;
-            if (++stage == C::kStages) {
-                stage = 0;
-                phase ^= 1u;
-            }
-        }
-    } else if (warp == 1 && lane == 0) {
-        // ---- MMA issuer: one accumulation of its own for every block of 128
-        int stage = 0;
-        unsigned phase = 0;
-        unsigned it = 0;
-        bool ok = true;
-        for (int tile = blockIdx.x; tile < ntiles && ok && !fp8_aborted(bar); tile += gridDim.x) {
-            for (int k = 0; k < nk; ++k, ++it) {
-                const unsigned buf = it & 1u;
-                if (!fp8_wait(&bar.tmem_empty[buf], ((it >> 1) & 1u) ^ 1u, bar, p.error_word) ||
-                    !fp8_wait(&bar.full[stage], phase, bar, p.error_word)) {
-                    ok = false;
-                    break;
-                }
-                tc_fence_after();
-                const uint32_t a0 = smem_addr(sm.a[stage]), b0 = smem_addr(sm.b[stage]);
+        } else if (warp == 1 && lane == 0) {
+            // ---- MMA issuer: one accumulation of its own for every block of 128.
+            // Instruction descriptor, kind::f8f6f4: fp32 accumulator (bits 4-5 = 1), A and B e4m3
+            // (bits 7-9, 10-12 = 0), both K-major (bits 15, 16 = 0), N >> 3 in bits 17-22, M >> 4 in
+            // bits 24-28.
+            constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(NC >> 3) << 17) | ((uint32_t)(kFM >> 4) << 24);
+            const uint64_t da0 = smem_desc_sw128(smem_addr(sm.a[0])), db0 = smem_desc_sw128(smem_addr(sm.b[0]));
+            unsigned stage = 0, phase = 0, it = 0;
+            bool ok = true;
+            for (int tile = blockIdx.x; tile < ntiles && ok && !fp8_aborted(sm); tile += gridDim.x) {
+                for (int k = 0; k < nk; ++k, ++it) {
+                    const unsigned buf = it & 1u, turn = it >> 1 & 1u;
+                    if (!fp8_wait(&sm.tmem_empty[buf], turn ^ 1u, sm, p.error_word) ||
+                        !fp8_wait(&sm.full[stage], phase, sm, p.error_word)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint64_t da = da0 + stage * (kFABytes >> 4), db = db0 + stage * (kFBBytes >> 4);
 #pragma unroll
-                for (int kk = 0; kk < kFK / 32; ++kk)  // 32 e4m3 = 32 bytes inside the swizzled 128-byte row
-                    tc_mma_fp8(tmem + buf * NT, smem_desc_sw128(a0 + kk * 32), smem_desc_sw128(b0 + kk * 32),
-                               C::kIdesc, kk != 0 ? 1u : 0u);
-                tc_commit(&bar.empty[stage]);
-                tc_commit(&bar.tmem_full[buf]);
-                if (++stage == C::kStages) {
-                    stage = 0;
-                    phase ^= 1u;
+                    for (int kk = 0; kk < kFK / 32; ++kk)  // 32 bytes (2 in the descriptor) on inside the swizzled 128-byte row
+                        tc_mma_fp8(tmem + buf * kFN, da + 2 * kk, db + 2 * kk, idesc, kk != 0);
+                    tc_commit(&sm.tmem_full[buf]);
+                    tc_commit(&sm.empty[stage]);
+                    if (++stage == kFStages) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
                 }
             }
+            // every MMA this thread issued is complete before TMEM is released
+            tc_commit(&sm.drain);
+            mbar_wait_bounded(&sm.drain, 0);
         }
-        // every MMA this thread issued is complete before TMEM is released
-        tc_commit(&bar.drain);
-        mbar_wait_bounded(&bar.drain, 0);
-    }
     } else {
-        if (C::kGroups == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         // ---- fold: warp w reads TMEM lanes 32 * (w % 4) .. +31
-        const int q = warp & 3;
-        const int col0 = ((warp - 4) >> 2) * C::kCols;
-        constexpr int kPart = C::kCols >= 64 ? 32 : 16;             // columns of one TMEM load
-        constexpr int kTwo = C::kCols >= 2 * kPart ? 2 : 1;         // loads in flight
-        float* const out = sm.out + (C::kStaged ? (warp - 4) * 1024 : 0);
-        unsigned it = 0;
-        bool ok = true;
-        for (int tile = blockIdx.x; tile < ntiles && ok; tile += gridDim.x) {
-            int mb, nb;
-            coords(tile, mb, nb);
-            const int in_tile = q * 32 + lane;
-            const int row = mb * p.tile_rows + in_tile;  // row of the operand on the lanes
-            const bool row_ok = in_tile < p.tile_rows && row < rows_a;
-            unsigned long long acc[C::kCols / 2];
-#pragma unroll
-            for (int j = 0; j < C::kCols / 2; ++j) acc[j] = 0ull;
-            const int wcol = nb * NT + col0;  // first of this thread's columns (of W, when W is not on the lanes)
-            const float* own_scale = kWLanes ? p.w_scales + (long long)(row / kFK) * nk : p.h_scales + (long long)row * nk;
-            const float* tile_scale = p.w_scales + (long long)(wcol / kFK) * nk;
-            const bool col_ok = kWLanes || wcol < p.vocab;
-            const auto scale_of = [&](int k) {
-                float s = row_ok && col_ok ? __ldg(own_scale + k) : 0.0f;
-                if (!kWLanes && row_ok && col_ok) s *= __ldg(tile_scale + k);
-                return s;
-            };
-            float s = scale_of(0);
-            for (int k = 0; k < nk; ++k, ++it) {
-                const unsigned buf = it & 1u;
-                const float s_next = k + 1 < nk ? scale_of(k + 1) : 0.0f;
-                const bool got = fp8_wait(&bar.tmem_full[buf], (it >> 1) & 1u, bar, p.error_word);
-                if (!__all_sync(kFullMask, got ? 1 : 0) || fp8_aborted(bar)) {
-                    ok = false;
-                    break;
-                }
-                tc_fence_after();
-                const uint32_t src = tmem + ((uint32_t)(q * 32) << 16) + buf * NT + (uint32_t)col0;
-                const unsigned long long ss = pair_of(s, s);
-#pragma unroll
-                for (int c = 0; c < C::kCols; c += kTwo * kPart) {
-                    uint32_t t[kTwo][kPart];
-#pragma unroll
-                    for (int h = 0; h < kTwo; ++h) tmem_load(src + (uint32_t)(c + h * kPart), t[h]);
-#pragma unroll
-                    for (int h = 0; h < kTwo; ++h) tmem_wait(t[h]);
-                    if (c + kTwo * kPart >= C::kCols) {  // the buffer has been read
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&bar.tmem_empty[buf]);
-                    }
-#pragma unroll
-                    for (int h = 0; h < kTwo; ++h)
-#pragma unroll
-                        for (int j = 0; j < kPart; j += 2) {
-                            const int at = c + h * kPart + j;
-                            unsigned long long f = ss;
-                            if (kWLanes) {
-                                const float2 hs = *reinterpret_cast<const float2*>(hs_sm + k * NT + at);
-                                f = pair_of(s * hs.x, s * hs.y);
-                            }
-                            fold2(acc[at / 2], t[h][j], t[h][j + 1], f);
-                        }
-                }
-                s = s_next;
-            }
-            ok = __all_sync(kFullMask, ok ? 1 : 0);
-            if (!ok) break;
-            if (kWLanes) {  // a lane per vocabulary entry: 32 consecutive logits of a row per store
-#pragma unroll
-                for (int j = 0; j < C::kCols; ++j) {
-                    const int b = nb * NT + j;
-                    const float2 v = halves_of(acc[j / 2]);
-                    if (row_ok && b < p.batch) store_logit(p, (long long)b * p.ld + row, (j & 1) ? v.y : v.x);
-                }
-            } else {
-                // 32 columns at a time through the warp's 32 x 32 floats; the 16-byte piece j of
-                // row r is at piece j ^ (r % 8), so neither side meets bank conflicts
-                float4* const out4 = reinterpret_cast<float4*>(out);
-                const int row0 = row - lane;
-#pragma unroll
-                for (int c = 0; c < C::kCols; c += 32) {
-                    __syncwarp();
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const float2 a = halves_of(acc[c / 2 + 2 * j]), b = halves_of(acc[c / 2 + 2 * j + 1]);
-                        out4[lane * 8 + (j ^ (lane & 7))] = make_float4(a.x, a.y, b.x, b.y);
-                    }
-                    __syncwarp();
-                    write_block(p, out, row0, wcol + c, lane);
-                }
-            }
-        }
+        if (NC > kFCols || warp < 8) fold_tiles<NC>(p, sm, tmem, mt, nt, nk);
     }
     tc_fence_before();
     __syncthreads();
     if (warp == 2) {
         tc_fence_after();
-        tmem_dealloc(tmem, C::kTmemCols);
+        tmem_dealloc(tmem, kFTmemCols);
     }
 }
 
@@ -430,50 +424,52 @@ bool make_tmap_fp8(CUtensorMap* m, const void* base, int rows, int dim, int box_
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int NT, bool kWLanes>
-cudaError_t launch_fp8(Fp8GemmLaunch p, int num_sms, cudaStream_t stream) {
-    using C = Fp8Cfg<NT, kWLanes>;
-    const void* a = kWLanes ? p.w : p.h;
-    const void* b = kWLanes ? p.h : p.w;
-    const int rows_a = kWLanes ? p.vocab : p.batch, rows_b = kWLanes ? p.batch : p.vocab;
-    p.tile_rows = kFM;
-    if (kWLanes) {  // as many tiles an SM as 128 rows each would take, of equal height
-        const int rounds = (rows_a + kFM * num_sms - 1) / (kFM * num_sms);
-        p.tile_rows = (rows_a + rounds * num_sms - 1) / (rounds * num_sms);
-    }
-    p.vec_out = (reinterpret_cast<uintptr_t>(p.logits) & 15u) == 0 && p.ld % (p.out_bf16 ? 8 : 4) == 0;
-    CUtensorMap ta, tb;
-    if (!make_tmap_fp8(&ta, a, rows_a, p.dim, p.tile_rows) || !make_tmap_fp8(&tb, b, rows_b, p.dim, NT))
+template <int NC>
+cudaError_t launch_fp8(const Fp8GemmLaunch& p, int num_sms, cudaStream_t stream) {
+    CUtensorMap th, tw;
+    if (!make_tmap_fp8(&th, p.h, p.batch, p.dim, p.box_rows) || !make_tmap_fp8(&tw, p.w, p.vocab, p.dim, NC))
         return cudaErrorInvalidValue;
-    const int nk = (p.dim + kFK - 1) / kFK;
-    const size_t smem = sizeof(Fp8Smem<NT, kWLanes>) + 1024 + (kWLanes ? (size_t)nk * NT * sizeof(float) : 0);
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     static std::atomic<unsigned long long> attr_done{0};
     const unsigned long long bit = 1ull << (dev & 63);
     if (!(attr_done.load() & bit)) {
-        e = cudaFuncSetAttribute(fp8_gemm_kernel<NT, kWLanes>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 kFp8MaxSmem);
+        e = cudaFuncSetAttribute(fp8_gemm_kernel<NC>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kFp8SmemBytes);
         if (e != cudaSuccess) return e;
         attr_done.fetch_or(bit);
     }
-    const long long tiles = (long long)((rows_a + p.tile_rows - 1) / p.tile_rows) * ((rows_b + NT - 1) / NT);
+    const long long tiles = (long long)((p.batch + kFM - 1) / kFM) * ((p.vocab + NC - 1) / NC);
     const int grid = tiles < num_sms ? (int)tiles : num_sms;
-    fp8_gemm_kernel<NT, kWLanes><<<grid, C::kThreads, smem, stream>>>(ta, tb, p);
+    fp8_gemm_kernel<NC><<<grid, kFThreads, kFp8SmemBytes, stream>>>(th, tw, p);
     return cudaGetLastError();
 }
 
 }  // namespace
 
-int launch_fp8_gemm(const Fp8GemmLaunch& p, int num_sms, cudaStream_t stream) {
-    const int nk = (p.dim + kFK - 1) / kFK;
+int launch_fp8_gemm(const Fp8GemmLaunch& args, int num_sms, cudaStream_t stream) {
+    Fp8GemmLaunch p = args;
+    p.box_rows = p.batch < kFM ? (p.batch + 7) / 8 * 8 : kFM;
+    p.vec_out = (reinterpret_cast<uintptr_t>(p.logits) & 15u) == 0 && p.ld % (p.out_bf16 ? 8 : 4) == 0;
+    // Columns of a tile: such that the rounds of tiles that an SM goes through, each as long as its
+    // columns (and some 64 more: a block's way through the buffers), are shortest.
+    const long long mt = (p.batch + kFM - 1) / kFM;
+    long long best = 0;
+    int cols = kFN;
+    for (int c = kFN; c >= kFCols; c -= 32) {
+        const long long tiles = mt * ((p.vocab + c - 1) / c);
+        const long long cost = (tiles + num_sms - 1) / num_sms * (c + 64);
+        if (best == 0 || cost < best) {
+            best = cost;
+            cols = c;
+        }
+    }
     cudaError_t e;
-    // W on the lanes while the padded batch is one column tile and H's scales fit behind the ring.
-    if (p.batch <= 16 && nk <= 512) e = launch_fp8<16, true>(p, num_sms, stream);
-    else if (p.batch <= 32 && nk <= 256) e = launch_fp8<32, true>(p, num_sms, stream);
-    else if (p.batch <= 64 && nk <= 128) e = launch_fp8<64, true>(p, num_sms, stream);
-    else e = launch_fp8<256, false>(p, num_sms, stream);
+    if (cols == 256) e = launch_fp8<256>(p, num_sms, stream);
+    else if (cols == 224) e = launch_fp8<224>(p, num_sms, stream);
+    else if (cols == 192) e = launch_fp8<192>(p, num_sms, stream);
+    else if (cols == 160) e = launch_fp8<160>(p, num_sms, stream);
+    else e = launch_fp8<128>(p, num_sms, stream);
     return e == cudaSuccess ? 1 : -(int)e;
 }
 

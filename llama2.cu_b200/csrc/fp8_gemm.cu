@@ -154,18 +154,27 @@ __device__ __forceinline__ void write_block(const Fp8GemmLaunch& p, const T* out
         for (int r = 0; r < 32; ++r)
             if (r < rows && lane < n) to[r * p.ld + lane] = at(r, lane);
     } else {
-#pragma unroll 4
-        for (int r = 0; r < 32; ++r) {
-            if (r >= rows) break;
-            T* const q = to + r * p.ld;
+        // rows of one parity start alike: their pairs from column `odd` on, then the single
+        // columns that are left at either end, a lane a row
+#pragma unroll
+        for (int par = 0; par < 2; ++par) {
+            T* q = to + par * p.ld;
             const int odd = (int)(reinterpret_cast<uintptr_t>(q) >> 1 & 1u), c = 2 * lane + odd;
-            if (c + 1 < n) {
-                T pair[2] = {at(r, c), at(r, c + 1)};
-                *reinterpret_cast<uint32_t*>(q + c) = *reinterpret_cast<const uint32_t*>(pair);
-            } else if (c < n) {
-                q[c] = at(r, c);
-            }
-            if (odd && lane == 0) q[0] = at(r, 0);
+            const bool there = c + 1 < n;
+            const long long step = 2 * p.ld;
+            q += c;
+#pragma unroll 8
+            for (int r = par; r < 32; r += 2, q += step)
+                if (r < rows && there) {
+                    T pair[2] = {at(r, c), at(r, c + 1)};
+                    *reinterpret_cast<uint32_t*>(q) = *reinterpret_cast<const uint32_t*>(pair);
+                }
+        }
+        if (lane < rows) {
+            T* const q = to + lane * p.ld;
+            const int odd = (int)(reinterpret_cast<uintptr_t>(q) >> 1 & 1u);
+            if (odd) q[0] = at(lane, 0);
+            if ((n - odd) & 1) q[n - 1] = at(lane, n - 1);
         }
     }
 }

@@ -307,7 +307,7 @@ constexpr int kBinCap = 2048;      // bins of a histogram
 constexpr int kChunkBins = 512;    // bins of the chunk maxima
 constexpr int kChunkCap = 2048;    // chunk maxima kept: 64 groups of batches, one a lane
 constexpr int kU = 4;              // vectors of a lane in a batch
-constexpr int kWarpList = 64;      // a list of up to this many is one warp's work
+constexpr int kShortList = 128;    // a list of up to this many is put in order by counting
 constexpr float kLowest = -3.402823466e38f;
 
 template <int NT>
@@ -560,7 +560,7 @@ enum { kDone = 0, kNeedSum64 = 1, kNeedBins = 2, kNeedExact = 3 };
 // steps; the mean of |log2 w| under the weights is H - log2 S <= log2(V / S) bits.
 // Sums of trees are fp64.
 template <int NT, typename T, bool kLow>
-__device__ __forceinline__ void first_pass(const VecRow<T>& row, int shift, uint4 (&next)[kU], FastSmem<NT>& sm,
+__device__ __forceinline__ void first_pass(const VecRow<T>& row, int shift, uint4 (&raw)[kU], FastSmem<NT>& sm,
                                            RowFacts& f) {
     constexpr int E = VecRow<T>::E;
     constexpr int NW = NT / 32;
@@ -574,12 +574,8 @@ __device__ __forceinline__ void first_pass(const VecRow<T>& row, int shift, uint
     double run_sum = 0.0;
     int b = warp << shift;
     while (b < row.batches) {
-        uint4 raw[kU];
-#pragma unroll
-        for (int u = 0; u < kU; ++u) raw[u] = next[u];
         const int now = b;
         b = ((b + 1) & group) ? b + 1 : b + 1 + ((NW - 1) << shift);
-        if (b < row.batches) row.load_batch(b, lane, next);  // on its way while this one is used
         float m = -inf;
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
@@ -630,6 +626,7 @@ __device__ __forceinline__ void first_pass(const VecRow<T>& row, int shift, uint
         float a, c;
         unpack2(add2(add2(t[0], t[1]), add2(t[2], t[3])), a, c);
         run_sum += (double)(a + c);
+        if (b < row.batches) row.load_batch(b, lane, raw);
     }
     // all of these are a lane's; then a warp's; then the row's, in every warp
     top = warp_max_nan(top);
@@ -787,14 +784,32 @@ __device__ void scan_list(const u64* list, double* cum, int n, double base, cons
     __syncthreads();
 }
 
-// The same two for a list of up to kWarpList keys, by one warp.
-__device__ __forceinline__ void sort_and_scan_warp(u64* list, double* cum, int n, const RowFacts& f, int lane) {
-    if (n <= 32) warp_sort_desc<1>(list, n, lane);
-    else warp_sort_desc<kWarpList / 32>(list, n, lane);
-    __syncwarp();
+// A list of up to kShortList keys in order, each at the number of keys above it
+// (counted by NT / kShortList or twice as many threads a key), behind the list;
+// its weights in the same order.
+template <int NT>
+__device__ __forceinline__ const u64* order_short_list(u64* list, double* weight, int n, const RowFacts& f) {
+    const int parts = n <= kShortList / 2 ? NT / (kShortList / 2) : NT / kShortList;
+    const int i = (int)threadIdx.x / parts, part = (int)threadIdx.x % parts;
+    u64* sorted = list + kListCap / 2;
+    const u64 key = i < n ? list[i] : 0ull;
+    int above = 0;
+    if (i < n)
+        for (int j = part; j < n; j += parts) above += list[j] > key;
+    for (int o = parts >> 1; o; o >>= 1) above += __shfl_xor_sync(kFullMask, above, o);
+    if (i < n && part == 0) {
+        sorted[above] = key;
+        weight[above] = f.weight(key_value((uint32_t)(key >> 32)));
+    }
+    __syncthreads();
+    return sorted;
+}
+
+// Weights into their running sums, by one warp.
+__device__ __forceinline__ void scan_warp(double* cum, int n, int lane) {
     double before = 0.0;
     for (int i = lane; i - lane < n; i += 32) {
-        double c = i < n ? f.weight(key_value((uint32_t)(list[i] >> 32))) : 0.0;
+        double c = i < n ? cum[i] : 0.0;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const double u = __shfl_up_sync(kFullMask, c, o);
@@ -834,10 +849,9 @@ __device__ __forceinline__ void write_row(const FilterLaunch& p, int r, u64 key,
 // not reach far enough, kNeedSum64 when `sum`, off by up to err, leaves a border
 // open.  `complete`: every candidate is listed.
 template <int NT>
-__device__ int decide_list(const FilterLaunch& p, int r, const RowRule& rule, const RowFacts& f, int n, bool complete,
-                           int k, double sum, double err, int candidates, FastSmem<NT>& sm) {
+__device__ int decide_list(const FilterLaunch& p, int r, const RowRule& rule, const RowFacts& f, const u64* key, int n,
+                           bool complete, int k, double sum, double err, int candidates, FastSmem<NT>& sm) {
     const int lane = threadIdx.x & 31;
-    const u64* key = sm.list.key;
     const double* cum = sm.list.cum;
     const bool use_p = rule.topp > 0.0f && rule.topp < 1.0f;
     const bool listed = k > 0 || rule.minp > 0.0f || complete;  // the mass that top-p and the draw refer to
@@ -948,32 +962,34 @@ __device__ __forceinline__ int sample_from_list(const FilterLaunch& p, int r, co
     // entries to expect, were they spread over the chunks at random
     const float g = (float)f.chunks;
     const float expect = hits < f.chunks ? -g * __logf(1.0f - (float)hits / g) : 1e9f;
-    if (row.vocab <= kListCap && expect > 0.3f * kListCap) {
+    if (row.vocab <= kShortList) {  // the whole row is a short list
         cut = -inf;
         hits = f.chunks;
         __syncthreads();
         for (int c = threadIdx.x; c < f.chunks; c += NT) sm.list.hit[c] = c;
         __syncthreads();
-    } else if (expect > 0.9f * kListCap) {
-        return kNeedBins;
+    } else if (expect > fminf(0.9f * kListCap, 64.0f + 0.125f * (float)row.vocab)) {
+        return kNeedBins;  // too many for the list, or more to sort than the row is to read again
     }
     const bool complete = !(cut > -inf);
-    for (int i = threadIdx.x; i < hits; i += NT) {
-        const int c = sm.list.hit[i];
-        for (int j = 0; j <= (1 << f.chunk_shift) - 1; ++j) {
-            const int first = ((((c >> 5) << f.chunk_shift) + j) * kU << 5) | (c & 31);
-            uint4 raw[kU];
+    const int per = 2 + f.chunk_shift, items = hits << per;  // kU << chunk_shift vectors a chunk, one a thread
+    for (int i = threadIdx.x; i < items; i += 2 * NT) {
+        uint4 raw[2];
+        int vec[2];
 #pragma unroll
-            for (int u = 0; u < kU; ++u) raw[u] = row.load(first + 32 * u);
+        for (int u = 0; u < 2; ++u) {
+            const int it = i + u * NT, c = it < items ? sm.list.hit[it >> per] : 0;
+            vec[u] = it < items ? ((((c >> 5) << per) + (it & ((1 << per) - 1))) << 5) | (c & 31) : row.vecs;
+            raw[u] = row.load(vec[u]);
+        }
 #pragma unroll
-            for (int u = 0; u < kU; ++u) {
-                float v[E];
-                VecRow<T>::widen(raw[u], v);
-                unsigned mask = 0u;
+        for (int u = 0; u < 2; ++u) {
+            float v[E];
+            VecRow<T>::widen(raw[u], v);
+            unsigned mask = 0u;
 #pragma unroll
-                for (int e = 0; e < E; ++e) mask |= (v[e] >= cut && v[e] > -inf) ? 1u << e : 0u;
-                push_entries<T>(row, first + 32 * u, v, mask, sm.list.key, kListCap, &sm.n[0]);
-            }
+            for (int e = 0; e < E; ++e) mask |= (v[e] >= cut && v[e] > -inf) ? 1u << e : 0u;
+            push_entries<T>(row, vec[u], v, mask, sm.list.key, kListCap, &sm.n[0]);
         }
     }
     __syncthreads();
@@ -982,13 +998,16 @@ __device__ __forceinline__ int sample_from_list(const FilterLaunch& p, int r, co
     if (n > kListCap || n < 1 || (k > 0 && n < k && !complete && !all_of_minp)) return kNeedBins;
     int candidates = row.vocab;
     if (open && !use_p && !complete && !(f.low > -inf) && p.kept) candidates = count_candidates<NT>(row, sm);
-    if (n > kWarpList) {
+    const u64* key = sm.list.key;
+    if (n > kShortList) {
         sort_list<NT>(sm.list.key, n);
         scan_list<NT>(sm.list.key, sm.list.cum, n, 0.0, f, sm);
+    } else {
+        key = order_short_list<NT>(sm.list.key, sm.list.cum, n, f);
     }
     if (warp == 0) {
-        if (n <= kWarpList) sort_and_scan_warp(sm.list.key, sm.list.cum, n, f, lane);
-        const int st = decide_list<NT>(p, r, rule, f, n, complete, k, (double)f.sum, (double)f.sum * f.sum_err,
+        if (n <= kShortList) scan_warp(sm.list.cum, n, lane);
+        const int st = decide_list<NT>(p, r, rule, f, key, n, complete, k, (double)f.sum, (double)f.sum * f.sum_err,
                                        candidates, sm);
         if (lane == 0) sm.status = st;
     }
@@ -996,7 +1015,7 @@ __device__ __forceinline__ int sample_from_list(const FilterLaunch& p, int r, co
     if (sm.status != kNeedSum64) return sm.status;
     const double s64 = sum64<NT>(row, f, sm);
     if (warp == 0) {
-        const int st = decide_list<NT>(p, r, rule, f, n, complete, k, s64, 0.0, candidates, sm);
+        const int st = decide_list<NT>(p, r, rule, f, key, n, complete, k, s64, 0.0, candidates, sm);
         if (lane == 0) sm.status = st;
     }
     __syncthreads();
@@ -1288,8 +1307,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) filtered_sample_kernel(FilterLa
     const VecRow<T> row(static_cast<const T*>(p.logits) + (long long)r * p.ld, p.vocab);
     int shift = 0;
     while (((row.batches - 1) >> shift) >= kChunkCap / 32) ++shift;
-    uint4 next[kU];  // on their way while the settings are read
-    if ((threadIdx.x >> 5) << shift < row.batches) row.load_batch((threadIdx.x >> 5) << shift, threadIdx.x & 31, next);
+    uint4 raw[kU];  // the first batch is on its way while the settings are read
+    if ((threadIdx.x >> 5) << shift < row.batches) row.load_batch((threadIdx.x >> 5) << shift, threadIdx.x & 31, raw);
     RowRule rule = row_rule(p, r, threadIdx.x == 0);
     for (int i = threadIdx.x; i < kChunkBins; i += NT) sm.chunk_bin[i] = 0u;
     if (threadIdx.x == 0) {
@@ -1302,8 +1321,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) filtered_sample_kernel(FilterLa
     f.z = (float)f.z64;
     const int k = rule.topk > 0 && rule.topk < p.vocab ? rule.topk : 0;
     const bool open = !rule.greedy && k == 0 && !(rule.minp > 0.0f) && !(rule.topp > 0.0f && rule.topp < 1.0f);
-    if (open) first_pass<NT, T, true>(row, shift, next, sm, f);
-    else first_pass<NT, T, false>(row, shift, next, sm, f);
+    if (open) first_pass<NT, T, true>(row, shift, raw, sm, f);
+    else first_pass<NT, T, false>(row, shift, raw, sm, f);
     rule.coin = sm.coin;
     const bool plain = f.top > -__int_as_float(0x7F800000) && f.top < __int_as_float(0x7F800000);  // and no NaN
     int st = kNeedExact;
@@ -1324,10 +1343,15 @@ __global__ void __launch_bounds__(NT, 1024 / NT) filtered_sample_kernel(FilterLa
 
 template <typename T>
 void launch_rows(const FilterLaunch& p, int num_sms, cudaStream_t stream) {
-    // Up to two rows an SM: all of an SM's threads on one row, for the row's
-    // latency.  More: several rows at a time on an SM, whose passes overlap.
-    if (p.batch <= 2 * num_sms) filtered_sample_kernel<1024, T><<<p.batch, 1024, 0, stream>>>(p);
-    else filtered_sample_kernel<256, T><<<p.batch, 256, 0, stream>>>(p);
+    // Threads of a row.  Up to two rows an SM: enough of them that a warp has a batch
+    // or two, for the row's latency.  More rows: several on an SM at a time, whose
+    // passes overlap; a row of at most 16 batches leaves 8 warps too little between
+    // their barriers (4096 x 6000 bf16: 97 us with 8 warps, 68 with 4).
+    const long long batches = ((long long)p.vocab * sizeof(T) + 2047) / 2048;
+    const bool few = p.batch <= 2 * num_sms;
+    if (few && batches > 16) filtered_sample_kernel<1024, T><<<p.batch, 1024, 0, stream>>>(p);
+    else if (few || batches > 16) filtered_sample_kernel<256, T><<<p.batch, 256, 0, stream>>>(p);
+    else filtered_sample_kernel<128, T><<<p.batch, 128, 0, stream>>>(p);
 }
 
 }  // namespace

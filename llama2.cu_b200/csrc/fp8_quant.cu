@@ -13,10 +13,14 @@
 //
 // All three are bound by memory: an element is read once (4 or 2 bytes) and
 // written once (1 byte).  What stands in the way is the number of instructions
-// an element costs, so a lane has eight consecutive elements (the scale, its
-// reciprocal and the addresses are worked out once for eight), the division is
-// a product and two FMAs, and the kernels come in two forms: kWhole, where every
-// group of eight is whole and aligned, and one that checks each element.
+// an element costs, so a lane has eight elements of one or two blocks (the scale,
+// its reciprocal and the addresses are worked out once for them), the division is
+// a product and two FMAs, and the kernels come in two forms.  kWhole, where rows
+// start on 16 bytes and have a multiple of eight columns: the eight are
+// consecutive, 16 lanes have a block's row.  Else they are four columns 32 apart of
+// one block's row, which the whole warp has, and four of another's, so that the
+// scalar loads and stores of a warp are of consecutive elements
+// (weights 20001 x 1601 fp16: 36 us, 64 with consecutive ones).
 #include "device_common.cuh"
 #include "fp8_filter_kernels.cuh"
 
@@ -42,9 +46,11 @@ struct Raw {
     uint32_t w[kN * sizeof(T) / 4];
 };
 
-// Eight elements from p, of which n exist (kWhole: all of them, or none when n <= 0).
+// Eight elements: consecutive from p, there when n > 0 (kWhole); else four from p
+// and four from p + second, 32 apart, of which those exist whose distance is below
+// n and n2.
 template <typename T, bool kWhole>
-__device__ __forceinline__ Raw<T> load_raw(const T* p, int n) {
+__device__ __forceinline__ Raw<T> load_raw(const T* p, int n, long long second, int n2) {
     constexpr int W = kN * sizeof(T) / 4;
     Raw<T> r;
 #pragma unroll
@@ -62,11 +68,13 @@ __device__ __forceinline__ Raw<T> load_raw(const T* p, int n) {
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < kN; ++i)
-            if (i < n) {
-                if (sizeof(T) == 4) r.w[i % W] = reinterpret_cast<const uint32_t*>(p)[i];
-                else r.w[i / 2] |= (uint32_t)reinterpret_cast<const unsigned short*>(p)[i] << (16 * (i & 1));
+        for (int i = 0; i < kN; ++i) {
+            const T* q = p + (i < 4 ? 0 : second) + (i & 3) * 32;
+            if ((i & 3) * 32 < (i < 4 ? n : n2)) {
+                if (sizeof(T) == 4) r.w[i % W] = __ldcs(reinterpret_cast<const uint32_t*>(q));
+                else r.w[i / 2] |= (uint32_t)__ldcs(reinterpret_cast<const unsigned short*>(q)) << (16 * (i & 1));
             }
+        }
     }
     return r;
 }
@@ -86,7 +94,7 @@ __device__ __forceinline__ uint32_t e4m3_pair(float a, float b) {
 }
 
 template <bool kWhole>
-__device__ __forceinline__ void store_fp8(uint8_t* p, int n, const float (&v)[kN]) {
+__device__ __forceinline__ void store_fp8(uint8_t* p, int n, long long second, int n2, const float (&v)[kN]) {
     const uint32_t lo = e4m3_pair(v[0], v[1]) | (e4m3_pair(v[2], v[3]) << 16);
     const uint32_t hi = e4m3_pair(v[4], v[5]) | (e4m3_pair(v[6], v[7]) << 16);
     if (kWhole) {
@@ -94,23 +102,27 @@ __device__ __forceinline__ void store_fp8(uint8_t* p, int n, const float (&v)[kN
     } else {
 #pragma unroll
         for (int i = 0; i < kN; ++i)
-            if (i < n) p[i] = (uint8_t)((i < 4 ? lo : hi) >> (8 * (i & 3)));
+            if ((i & 3) * 32 < (i < 4 ? n : n2))
+                p[(i < 4 ? 0 : second) + (i & 3) * 32] = (uint8_t)((i < 4 ? lo : hi) >> (8 * (i & 3)));
     }
 }
 
 // Largest magnitude as bits (NaN > infinity > every finite value): of eight fp32
 // numbers, and of eight elements as they are in memory, where two 16-bit ones
 // are compared at once, accumulated into m and turned into fp32 bits at the end.
-__device__ __forceinline__ uint32_t abs_max_bits(const float (&v)[kN]) {
+__device__ __forceinline__ uint32_t abs_max_bits(const float (&v)[kN], int first, int n) {
     uint32_t m = 0u;
 #pragma unroll
-    for (int i = 0; i < kN; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+    for (int i = 0; i < kN; ++i)
+        if (i >= first && i < first + n) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
     return m;
 }
 template <typename T>
-__device__ __forceinline__ uint32_t raw_abs_max(uint32_t m, const Raw<T>& r) {
+__device__ __forceinline__ uint32_t raw_abs_max(uint32_t m, const Raw<T>& r, int first, int n) {
+    constexpr int W = kN * (int)sizeof(T) / 4;
 #pragma unroll
-    for (int i = 0; i < kN * (int)sizeof(T) / 4; ++i) {
+    for (int i = 0; i < W; ++i) {
+        if (i < first * W / kN || i >= (first + n) * W / kN) continue;
         if (sizeof(T) == 4) m = max(m, r.w[i] & 0x7FFFFFFFu);
         else m = __vmaxu2(m, r.w[i] & 0x7FFF7FFFu);
     }
@@ -147,19 +159,47 @@ __device__ __forceinline__ float block_scale(uint32_t amax_bits) {
 // v[i] = RN(v[i] / s) in the same way.  With s in [2^-60, 2^60] no intermediate of
 // a v above 2^-12 s leaves the normal range, and a smaller v gives 0 either way
 // (half the smallest e4m3 value is 2^-10).
-__device__ __forceinline__ void divide_by_scale(float (&v)[kN], float s) {
+__device__ __forceinline__ void divide_by_scale(float (&v)[kN], float s, int first, int n) {
     if (s < 0x1p-60f || s > 0x1p60f) {  // both by the same power of two, into the range
         const float f = s < 1.0f ? 0x1p80f : 0x1p-80f;
         s *= f;
 #pragma unroll
-        for (int i = 0; i < kN; ++i) v[i] *= f;
+        for (int i = 0; i < kN; ++i)
+            if (i >= first && i < first + n) v[i] *= f;
     }
     const float r = __frcp_rn(s);
 #pragma unroll
-    for (int i = 0; i < kN; ++i) {
-        const float q = __fmul_rn(v[i], r);
-        v[i] = __fmaf_rn(__fmaf_rn(-q, s, v[i]), r, q);
+    for (int i = 0; i < kN; ++i)
+        if (i >= first && i < first + n) {
+            const float q = __fmul_rn(v[i], r);
+            v[i] = __fmaf_rn(__fmaf_rn(-q, s, v[i]), r, q);
+        }
+}
+
+// One row's 1 x 128 blocks: divides a lane's eight values by their blocks' scales,
+// of which the largest magnitudes (m of the first four or of all eight, m2 of the
+// last four) are this lane's, and writes the scales; `block` is the first block
+// that the lane has a part of, `there` and `there2` say whether it and the next exist.
+template <bool kWhole>
+__device__ __forceinline__ void scale_blocks(float (&v)[kN], uint32_t m, uint32_t m2, float* scale, bool there,
+                                             bool there2) {
+    const int lane = threadIdx.x & 31;
+    if (kWhole) {
+        const float s = block_scale(half_warp_max(m));
+        divide_by_scale(v, s, 0, kN);
+        if (lane % kG == 0 && there) *scale = s;
+    } else {
+        const float s = block_scale(__reduce_max_sync(kFullMask, m)), s2 = block_scale(__reduce_max_sync(kFullMask, m2));
+        divide_by_scale(v, s, 0, 4);
+        divide_by_scale(v, s2, 4, 4);
+        if (lane == 0 && there) scale[0] = s;
+        if (lane == 0 && there2) scale[1] = s2;
     }
+}
+// Column of a lane's first element in the 256 columns of a warp.
+template <bool kWhole>
+__device__ __forceinline__ int lane_column() {
+    return (int)(threadIdx.x & 31) * (kWhole ? kN : 1);
 }
 
 // ---- activations: 1 x 128 blocks -------------------------------------------------
@@ -168,26 +208,27 @@ template <typename T, bool kWhole>
 __global__ void __launch_bounds__(kQThreads)
     quantize_rows_kernel(const T* x, long long ld, unsigned items, unsigned segs, int dim, uint8_t* q, float* scales) {
     constexpr int kUnits = sizeof(T) == 4 ? 2 : 4;
-    const int lane = threadIdx.x & 31;
     const int nb = (dim + kQBlock - 1) / kQBlock;
     for (unsigned it = blockIdx.x * (kQThreads / 32) + (threadIdx.x >> 5); it < items; it += gridDim.x * (kQThreads / 32)) {
         const unsigned row = it / segs;
-        const int col = (int)(it - row * segs) * (kUnits * 32 * kN) + lane * kN;
+        const int col = (int)(it - row * segs) * (kUnits * 32 * kN) + lane_column<kWhole>();
         const T* xp = x + (long long)row * ld + col;
         uint8_t* qp = q + (long long)row * dim + col;
         Raw<T> raw[kUnits];
 #pragma unroll
-        for (int k = 0; k < kUnits; ++k)
-            raw[k] = load_raw<T, kWhole>(xp + k * 32 * kN, dim - col - k * 32 * kN);
+        for (int k = 0; k < kUnits; ++k) {
+            const int n = dim - col - k * 32 * kN;
+            raw[k] = load_raw<T, kWhole>(xp + k * 32 * kN, n, kQBlock, n - kQBlock);
+        }
 #pragma unroll
         for (int k = 0; k < kUnits; ++k) {
-            const int c = col + k * 32 * kN;
+            const int c = col + k * 32 * kN, n = dim - c;
             float v[kN];
             widen_raw(raw[k], v);
-            const float s = block_scale(half_warp_max(magnitude_bits<T>(raw_abs_max(0u, raw[k]))));
-            divide_by_scale(v, s);
-            if (lane % kG == 0 && c < dim) scales[(long long)row * nb + c / kQBlock] = s;
-            store_fp8<kWhole>(qp + k * 32 * kN, dim - c, v);
+            const uint32_t m = magnitude_bits<T>(raw_abs_max(0u, raw[k], 0, kWhole ? kN : 4));
+            const uint32_t m2 = kWhole ? 0u : magnitude_bits<T>(raw_abs_max(0u, raw[k], 4, 4));
+            scale_blocks<kWhole>(v, m, m2, scales + (long long)row * nb + c / kQBlock, n > 0, n > kQBlock);
+            store_fp8<kWhole>(qp + k * 32 * kN, n, kQBlock, n - kQBlock, v);
         }
     }
 }
@@ -198,22 +239,27 @@ __global__ void __launch_bounds__(kQThreads)
 template <typename T, bool kWhole>
 __global__ void __launch_bounds__(kQThreads, sizeof(T) == 4 ? 2 : 4)
     quantize_blocks_kernel(const T* x, long long ld, int rows, int dim, uint8_t* q, float* scales) {
-    constexpr int kRowsPer = kQThreads / kG;  // rows of one step
+    // rows of one step: 16 lanes a row, or a warp for a row and the one 8 below
+    constexpr int kRowsPer = kQThreads / kG;
     constexpr int kSteps = kQBlock / kRowsPer;
     __shared__ uint32_t red[kQThreads / 32];
     const int nb = (dim + kQBlock - 1) / kQBlock;
     const int br = blockIdx.x / nb, bc = blockIdx.x - br * nb;
-    const int col = bc * kQBlock + (threadIdx.x % kG) * kN;
-    const int row0 = br * kQBlock + threadIdx.x / kG;
+    const int col = bc * kQBlock + (kWhole ? (int)(threadIdx.x % kG) * kN : (int)(threadIdx.x & 31));
+    const int row0 = br * kQBlock + (int)threadIdx.x / (kWhole ? kG : 32);
     const T* xp = x + (long long)row0 * ld + col;
     uint8_t* qp = q + (long long)row0 * dim + col;
+    const int cols = min(dim, (bc + 1) * kQBlock) - col;  // of this block from `col` on
     Raw<T> raw[kSteps];
     uint32_t m = 0u;
 #pragma unroll
-    for (int k = 0; k < kSteps; ++k)
-        raw[k] = load_raw<T, kWhole>(xp + (long long)k * kRowsPer * ld, row0 + k * kRowsPer < rows ? dim - col : 0);
+    for (int k = 0; k < kSteps; ++k) {
+        const int row = row0 + k * kRowsPer;
+        raw[k] = load_raw<T, kWhole>(xp + (long long)k * kRowsPer * ld, row < rows ? cols : 0, 8 * ld,
+                                     row + 8 < rows ? cols : 0);
+    }
 #pragma unroll
-    for (int k = 0; k < kSteps; ++k) m = raw_abs_max(m, raw[k]);
+    for (int k = 0; k < kSteps; ++k) m = raw_abs_max(m, raw[k], 0, kN);
     m = __reduce_max_sync(kFullMask, magnitude_bits<T>(m));
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
     __syncthreads();
@@ -223,10 +269,11 @@ __global__ void __launch_bounds__(kQThreads, sizeof(T) == 4 ? 2 : 4)
     if (threadIdx.x == 0) scales[(long long)br * nb + bc] = s;
 #pragma unroll
     for (int k = 0; k < kSteps; ++k) {
+        const int row = row0 + k * kRowsPer;
         float v[kN];
         widen_raw(raw[k], v);
-        divide_by_scale(v, s);
-        store_fp8<kWhole>(qp + (long long)k * kRowsPer * dim, row0 + k * kRowsPer < rows ? dim - col : 0, v);
+        divide_by_scale(v, s, 0, kN);
+        store_fp8<kWhole>(qp + (long long)k * kRowsPer * dim, row < rows ? cols : 0, 8LL * dim, row + 8 < rows ? cols : 0, v);
     }
 }
 
@@ -241,8 +288,7 @@ __global__ void __launch_bounds__(kQThreads, kHeld <= 2 ? 5 : 3)
     rmsnorm_fp8_kernel(const T* x, long long ld, const float* weight, int dim, uint8_t* q, float* scales) {
     constexpr int kSpan = kQThreads * kN;  // elements of one step of the CTA
     __shared__ float red[kQThreads / 32];
-    const int j0 = (int)threadIdx.x * kN;
-    const int warp_j0 = j0 - (int)(threadIdx.x & 31) * kN;
+    const int warp_j0 = (int)(threadIdx.x >> 5) * 32 * kN, j0 = warp_j0 + lane_column<kWhole>();
     const int nb = (dim + kQBlock - 1) / kQBlock;
     const T* xr = x + (long long)blockIdx.x * ld + j0;
     uint8_t* qr = q + (long long)blockIdx.x * dim + j0;
@@ -256,10 +302,14 @@ __global__ void __launch_bounds__(kQThreads, kHeld <= 2 ? 5 : 3)
         for (int i = 0; i < kN; ++i) ss = __fmaf_rn(t[i], t[i], ss);
     };
 #pragma unroll
-    for (int k = 0; k < kHeld; ++k) raw[k] = load_raw<T, kWhole>(xr + k * kSpan, dim - j0 - k * kSpan);
+    for (int k = 0; k < kHeld; ++k) {
+        const int n = dim - j0 - k * kSpan;
+        raw[k] = load_raw<T, kWhole>(xr + k * kSpan, n, kQBlock, n - kQBlock);
+    }
 #pragma unroll
     for (int k = 0; k < kHeld; ++k) add_squares(raw[k]);
-    for (int j = kHeld * kSpan; j0 + j < dim; j += kSpan) add_squares(load_raw<T, kWhole>(xr + j, dim - j0 - j));
+    for (int j = kHeld * kSpan; j0 + j < dim; j += kSpan)
+        add_squares(load_raw<T, kWhole>(xr + j, dim - j0 - j, kQBlock, dim - j0 - j - kQBlock));
 #pragma unroll
     for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(kFullMask, ss, o);
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = ss;
@@ -269,7 +319,7 @@ __global__ void __launch_bounds__(kQThreads, kHeld <= 2 ? 5 : 3)
     for (int i = 0; i < kQThreads / 32; ++i) tot += red[i];
     const float r = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(tot, (float)dim), 1e-5f)));
     const auto finish = [&](const Raw<T>& raw8, int j) {
-        const int n = dim - j0 - j;  // elements that exist
+        const int n = dim - j0 - j;  // columns from the lane's first one on
         float t[kN], w[kN];
         widen_raw(raw8, t);
         const float* wp = weight + j0 + j;
@@ -281,28 +331,27 @@ __global__ void __launch_bounds__(kQThreads, kHeld <= 2 ? 5 : 3)
             }
             w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
             w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+#pragma unroll
+            for (int i = 0; i < kN; ++i) t[i] = __fmul_rn(w[i], __fmul_rn(r, t[i]));
+            if (n <= 0) {  // a column past the row is 0 whatever r is
+#pragma unroll
+                for (int i = 0; i < kN; ++i) t[i] = 0.0f;
+            }
         } else {
 #pragma unroll
-            for (int i = 0; i < kN; ++i) w[i] = i < n ? __ldg(wp + i) : 0.0f;
+            for (int i = 0; i < kN; ++i) {
+                const int at = (i & 3) * 32 + (i < 4 ? 0 : kQBlock);
+                t[i] = at < n ? __fmul_rn(__ldg(wp + at), __fmul_rn(r, t[i])) : 0.0f;
+            }
         }
-#pragma unroll
-        for (int i = 0; i < kN; ++i) t[i] = __fmul_rn(w[i], __fmul_rn(r, t[i]));
-        if (n < kN) {  // a column past the row is 0 whatever r is
-#pragma unroll
-            for (int i = 0; i < kN; ++i)
-                if (i >= n) t[i] = 0.0f;
-        }
-        const float s = block_scale(half_warp_max(abs_max_bits(t)));
-        divide_by_scale(t, s);
-        if (n > 0) {
-            if (threadIdx.x % kG == 0) sr[(j0 + j) / kQBlock] = s;
-            store_fp8<kWhole>(qr + j, n, t);
-        }
+        scale_blocks<kWhole>(t, abs_max_bits(t, 0, kWhole ? kN : 4), kWhole ? 0u : abs_max_bits(t, 4, 4),
+                             sr + (j0 + j) / kQBlock, n > 0, n > kQBlock);
+        store_fp8<kWhole>(qr + j, n, kQBlock, n - kQBlock, t);
     };
 #pragma unroll
     for (int k = 0; k < kHeld; ++k)
         if (warp_j0 + k * kSpan < dim) finish(raw[k], k * kSpan);  // whole warps: the maximum needs every lane
-    for (int j = kHeld * kSpan; warp_j0 + j < dim; j += kSpan) finish(load_raw<T, kWhole>(xr + j, dim - j0 - j), j);
+    for (int j = kHeld * kSpan; warp_j0 + j < dim; j += kSpan) finish(load_raw<T, kWhole>(xr + j, dim - j0 - j, kQBlock, dim - j0 - j - kQBlock), j);
 }
 
 bool aligned(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }

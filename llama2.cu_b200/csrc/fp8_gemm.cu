@@ -322,6 +322,11 @@ __global__ void __launch_bounds__(kFThreads, 1)
     const int ntiles = mt * nt;
     const int nk = (p.dim + kFK - 1) / kFK;
 
+    const auto load_stage = [&](unsigned stage, int k, int mb, int nb) {
+        mbar_arrive_expect_tx(&sm.full[stage], (unsigned)(p.box_rows + NC) * kFK);
+        tma_load_2d(sm.a[stage], &tmap_h, k * kFK, mb * kFM, &sm.full[stage]);
+        tma_load_2d(sm.b[stage], &tmap_w, k * kFK, nb * NC, &sm.full[stage]);
+    };
     if (tid == 0) {
         for (int s = 0; s < kFStages; ++s) {
             mbar_init(&sm.full[s], 1);
@@ -334,6 +339,10 @@ __global__ void __launch_bounds__(kFThreads, 1)
         mbar_init(&sm.drain, 1);
         sm.abort = 0;
         fence_mbar_init();
+        // the first stages are on their way while TMEM is allocated
+        int mb, nb;
+        fp8_tile_coords(blockIdx.x, mt, nt, mb, nb);
+        for (int k = 0; k < min(nk, kFStages); ++k) load_stage(k, k, mb, nb);
     }
     if (warp == 2) {
         tmem_alloc(smem_addr(&sm.tmem_base), kFTmemCols);
@@ -349,16 +358,15 @@ __global__ void __launch_bounds__(kFThreads, 1)
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         if (warp == 0 && lane == 0) {
             // ---- TMA producer
-            const unsigned bytes = (unsigned)(p.box_rows + NC) * kFK;
-            unsigned stage = 0, phase = 0;
-            for (int tile = blockIdx.x; tile < ntiles && !fp8_aborted(sm); tile += gridDim.x) {
+            const int ahead = min(nk, kFStages);  // issued above
+            unsigned stage = ahead == kFStages ? 0 : ahead, phase = ahead == kFStages ? 1 : 0;
+            int k = ahead;
+            for (int tile = blockIdx.x; tile < ntiles && !fp8_aborted(sm); tile += gridDim.x, k = 0) {
                 int mb, nb;
                 fp8_tile_coords(tile, mt, nt, mb, nb);
-                for (int k = 0; k < nk; ++k) {
+                for (; k < nk; ++k) {
                     if (!fp8_wait(&sm.empty[stage], phase ^ 1u, sm, p.error_word)) break;
-                    mbar_arrive_expect_tx(&sm.full[stage], bytes);
-                    tma_load_2d(sm.a[stage], &tmap_h, k * kFK, mb * kFM, &sm.full[stage]);
-                    tma_load_2d(sm.b[stage], &tmap_w, k * kFK, nb * NC, &sm.full[stage]);
+                    load_stage(stage, k, mb, nb);
                     if (++stage == kFStages) {
                         stage = 0;
                         phase ^= 1u;

@@ -282,7 +282,9 @@ int sampler_batched_noalloc(const SamplerBatchConfig* cfg, const float* logits, 
  * Filtered sampling and the 8-bit classifier (no counterpart in the
  * reference, whose sampler knows temperature and top-p over fp32 logits and
  * whose classifier is fp32 or 16-bit).  Device buffers; every call is
- * asynchronous on `stream` and can be captured into a CUDA graph.
+ * asynchronous on `stream`, allocates nothing and can be captured into a CUDA
+ * graph, once some call has been made on the device before (the first one sets
+ * up what the library keeps for a device).
  * ---------------------------------------------------------------------- */
 
 /* Element types of the 16- and 32-bit buffers below. */

@@ -369,6 +369,15 @@ def _block_matrix(t, what, rows, cols, dtype, device):
     return t.data_ptr()
 
 
+def _alloc(shape, dtype, device, stream):
+    """torch.empty in the order of the stream that will use it (a block of another
+    stream's could still be in use there)."""
+    if stream is None:
+        return _Torch.empty(shape, dtype=dtype, device=device)
+    with _Torch.torch.cuda.stream(stream):
+        return _Torch.empty(shape, dtype=dtype, device=device)
+
+
 def _on_device(device, rows, stream, name, *args):
     """Calls entry point `name` with the operands' device current, on `stream`
     (default: that device's current one); nothing for an empty batch, whose
@@ -404,8 +413,8 @@ def sample_filtered(logits, temperature, topk, topp, minp, rng_state=None, *, te
     code, B, V, ld, dev = _matrix(logits, "logits")
     f32, i32 = _Torch.f32, _Torch.i32
     if out_ids is None:
-        out_ids = _Torch.empty(B, dtype=i32, device=dev)
-    cfg = SamplerFilterConfig(V, code, temperature, topk, topp, minp)
+        out_ids = _alloc(B, i32, dev, stream)
+    cfg = SamplerFilterConfig(V, code, temperature, min(max(topk, 0), V), topp, minp)
     _on_device(dev, B, stream, "sampler_filtered", cfg, logits.data_ptr(), B, ld,
                _vector(temperature_rows, "temperature_rows", B, f32, dev),
                _vector(topk_rows, "topk_rows", B, i32, dev), _vector(topp_rows, "topp_rows", B, f32, dev),
@@ -416,15 +425,15 @@ def sample_filtered(logits, temperature, topk, topp, minp, rng_state=None, *, te
     return out_ids
 
 
-def _fp8_outputs(R, D, block_rows, dev, out, scales_out):
+def _fp8_outputs(R, D, block_rows, dev, out, scales_out, stream):
     rows, cols = -(-R // block_rows), (D + 127) // 128
     if out is None:
-        out = _Torch.empty((R, D), dtype=_Torch.f8, device=dev)
+        out = _alloc((R, D), _Torch.f8, dev, stream)
         qp = out.data_ptr()
     else:
         qp = _block_matrix(out, "out", R, D, _Torch.f8, dev)
     if scales_out is None:
-        scales_out = _Torch.empty((rows, cols), dtype=_Torch.f32, device=dev)
+        scales_out = _alloc((rows, cols), _Torch.f32, dev, stream)
         sp = scales_out.data_ptr()
     else:
         sp = _block_matrix(scales_out, "scales_out", rows, cols, _Torch.f32, dev)
@@ -438,7 +447,7 @@ def quantize_fp8(x, block_rows=1, *, out=None, scales_out=None, stream=None):
     code, R, D, ld, dev = _matrix(x, "x")
     if block_rows != 1 and block_rows != 128:
         raise SamplerError("block_rows must be 1 or 128")
-    out, scales_out, qp, sp = _fp8_outputs(R, D, block_rows, dev, out, scales_out)
+    out, scales_out, qp, sp = _fp8_outputs(R, D, block_rows, dev, out, scales_out, stream)
     _on_device(dev, R, stream, "quantize_fp8", x.data_ptr(), code, R, D, ld, block_rows, qp, sp)
     return out, scales_out
 
@@ -447,7 +456,7 @@ def rmsnorm_fp8(x, norm_weight, *, out=None, scales_out=None, stream=None):
     """quantize_fp8(norm_weight * x / rms(x)) with block_rows 1 in one pass: x
     float32, bfloat16 or float16 [B, D], norm_weight float32 [D]."""
     code, B, D, ld, dev = _matrix(x, "x")
-    out, scales_out, qp, sp = _fp8_outputs(B, D, 1, dev, out, scales_out)
+    out, scales_out, qp, sp = _fp8_outputs(B, D, 1, dev, out, scales_out, stream)
     _on_device(dev, B, stream, "rmsnorm_fp8", x.data_ptr(), code,
                _vector(norm_weight, "norm_weight", D, _Torch.f32, dev), B, D, ld, qp, sp)
     return out, scales_out
@@ -476,7 +485,7 @@ def classifier_logits_fp8(hidden, hidden_scales, wcls, wcls_scales, logits_out=N
     hsp = _block_matrix(hidden_scales, "hidden_scales", B, (D + 127) // 128, _Torch.f32, dev)
     V, wp, wsp = _fp8_weights(wcls, wcls_scales, D, dev)
     if logits_out is None:
-        logits_out = _Torch.empty((B, V), dtype=_Torch.f32, device=dev)
+        logits_out = _alloc((B, V), _Torch.f32, dev, stream)
     code, rows, cols, ld, out_dev = _matrix(logits_out, "logits_out")
     if rows != B or cols != V or out_dev != dev:
         raise SamplerError(f"logits_out must be [{B}, {V}] on {dev}")
@@ -505,13 +514,10 @@ def classifier_fp8_sample_filtered(x, norm_weight, wcls, wcls_scales, temperatur
             raise SamplerError("logits_out must be float32 or bfloat16")
         lp = _block_matrix(logits_out, "logits_out", B, V, logits_out.dtype, dev)
     n = lib().classifier_fp8_workspace_bytes(B, D, V, code if lp is None else -1)
-    # from torch's allocator: ordered on the stream, and a graph's own inside a capture
-    ws = _Torch.empty(n, dtype=_Torch.u8, device=dev)
-    if stream is not None:
-        ws.record_stream(stream)
+    ws = _alloc(n, _Torch.u8, dev, stream)  # from torch's allocator: inside a capture, the graph's own
     if out_ids is None:
-        out_ids = _Torch.empty(B, dtype=i32, device=dev)
-    cfg = SamplerFilterConfig(V, code, temperature, topk, topp, minp)
+        out_ids = _alloc(B, i32, dev, stream)
+    cfg = SamplerFilterConfig(V, code, temperature, min(max(topk, 0), V), topp, minp)
     _on_device(dev, B, stream, "classifier_fp8_sample_filtered", cfg, x.data_ptr(), x_code,
                _vector(norm_weight, "norm_weight", D, f32, dev), wp, wsp, B, D,
                _vector(temperature_rows, "temperature_rows", B, f32, dev),

@@ -839,7 +839,7 @@ int classifier_logits_fp8(const void* hidden, const float* hidden_scales, const 
     if (((uintptr_t)hidden_scales & 3u) || ((uintptr_t)wcls_scales & 3u) ||
         ((uintptr_t)logits_out & (dtype_size(logits_dtype) - 1)))
         return fail(SAMPLER_E_INVALID, "scales or logits_out not aligned to its elements");
-    if (((long long)batch + 127) / 128 * (((long long)vocab + 15) / 16) > 0x3FFFFFFFLL)
+    if (vocab > (1 << 30) || ((long long)batch + 127) / 128 * (((long long)vocab + 127) / 128) > 0x3FFFFFFFLL)
         return fail(SAMPLER_E_UNSUPPORTED, "batch %d by vocab %d is too large for one call", batch, vocab);
     if (batch == 0) return SAMPLER_OK;
     DeviceCtx* c = nullptr;

@@ -251,6 +251,16 @@ def test_temperatures(pkg, T):
 
 
 @pytest.mark.gpu
+def test_top_k_beyond_32_bits_is_off(pkg):
+    x = rows("peaked", 3, 2001, 6).cuda()
+    c = torch.from_numpy(coins_of(3, 2)).cuda()
+    kept = torch.empty(3, dtype=torch.int32, device="cuda")
+    for k in (2 ** 32 + 1, 2 ** 40, -2 ** 40):
+        pkg.sample_filtered(x, 1.0, k, 1.0, 0.0, coins=c, kept_out=kept)
+        assert kept.tolist() == [2001] * 3
+
+
+@pytest.mark.gpu
 def test_nan_settings_are_off(pkg):
     x = rows("peaked", 4, 3001, 2).cuda()
     nan = float("nan")

@@ -388,7 +388,7 @@ def test_c_refusals_before_any_device_work(pkg):
     assert [gemm(h=None), gemm(hs=None), gemm(w=None), gemm(ws=None), gemm(out=None), gemm(b=-1), gemm(d=8),
             gemm(d=100), gemm(v=0), gemm(ld=99), gemm(dt=2), gemm(h=A + 8), gemm(w=A + 8), gemm(hs=A + 2),
             gemm(out=A + 2)] == [-1] * 15
-    assert gemm(d=1 << 17) == -2
+    assert gemm(d=1 << 17) == -2 and gemm(v=(1 << 30) + 1, ld=1 << 31) == -2
     assert gemm(b=0) == 0
 
     cfg = pkg.SamplerFilterConfig(100, 0, 1.0, 0, 1.0, 0.0)

@@ -21,6 +21,8 @@
 // one block's row, which the whole warp has, and four of another's, so that the
 // scalar loads and stores of a warp are of consecutive elements
 // (weights 20001 x 1601 fp16: 36 us, 64 with consecutive ones).
+// Measured (1 B200): weights 32000 x 4096 bf16 62 us on the device (60 of bytes),
+// RMSNorm 8192 x 4096 fp32 35 us (26 of bytes).
 #include "device_common.cuh"
 #include "fp8_filter_kernels.cuh"
 

@@ -319,6 +319,7 @@ constexpr int kBinCap = 2048;      // bins of a histogram
 constexpr int kChunkBins = 512;    // bins of the chunk maxima
 constexpr int kChunkCap = 2048;    // chunk maxima kept: 64 groups of batches, one a lane
 constexpr int kU = 4;              // vectors of a lane in a batch
+constexpr int kFewChunks = 192;    // chunks of the second try of pass 2
 constexpr int kShortList = 128;    // a list of up to this many is put in order by counting
 constexpr float kLowest = -3.402823466e38f;
 
@@ -882,6 +883,57 @@ __device__ int decide_list(const FilterLaunch& p, int r, const RowRule& rule, co
     return kDone;
 }
 
+// A threshold by number where the one by mass asks for too long a list: heavy entries
+// that share a chunk are missing from the mass of the maxima, which then reaches for
+// entries far below them.  The kFewChunks largest maxima, if these nearly hold `mass`:
+// their chunks are listed and the threshold is returned, else NaN.  About 1 peaked
+// row in 1300 is such a one.  For the kernel of few rows, where one of them is the call's
+// time (64 x 128000 bf16, top-p: 104 us by the bins, 29 so); with many rows they hide
+// behind the others, and the tries of the rest cost more (4096 x 32000 222 -> 232 us).
+template <int NT>
+__device__ __noinline__ float cut_by_number(int chunks, float top, float low_chunk, float z, float mass,
+                                            FastSmem<NT>& sm) {
+    const int lane = threadIdx.x & 31;
+    const float inf = __int_as_float(0x7F800000);
+    const float scale = (float)(kChunkBins - 1) / (top - low_chunk);
+    __syncthreads();
+    for (int i = threadIdx.x; i < kChunkBins; i += NT) sm.chunk_bin[i] = 0u;
+    if (threadIdx.x == 0) sm.hits = 0u;
+    __syncthreads();
+    for (int i = threadIdx.x; i < chunks; i += NT) {
+        const float m = sm.chunk_max[i];
+        if (m > -inf) atomicAdd(&sm.chunk_bin[min((int)((top - m) * scale), kChunkBins - 1)], 1u);
+    }
+    __syncthreads();
+    constexpr int R = kChunkBins / 32;  // every warp forms the same threshold
+    unsigned c = 0;
+    for (int j = 0; j < R; ++j) c += sm.chunk_bin[lane * R + j];
+    unsigned ci = c;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned cu = __shfl_up_sync(kFullMask, ci, o);
+        if (lane >= o) ci += cu;
+    }
+    ci -= c;
+    int found = kChunkBins;
+    for (int j = 0; j < R; ++j) {
+        ci += sm.chunk_bin[lane * R + j];
+        if (ci >= kFewChunks && found == kChunkBins) found = lane * R + j;
+    }
+    found = __reduce_min_sync(kFullMask, found);
+    const float cut = __fsub_rd(top, ((float)found + 1.01f) / scale);
+    float held = 0.0f;
+    for (int i = threadIdx.x; i < chunks; i += NT) {
+        const float m = sm.chunk_max[i];
+        if (m >= cut) {
+            held += ex2_approx((m - top) * z);
+            sm.list.hit[atomicAdd(&sm.hits, 1u)] = i;
+        }
+    }
+    const double all = block_sum<NT>((double)held, sm.red_d);
+    return all >= 0.75 * (double)mass && sm.hits <= 2 * kFewChunks ? cut : __int_as_float(0x7FC00000);
+}
+
 // Pass 2: a threshold below which nothing can be kept or drawn, and the row
 // decided by the list of the entries above it.
 template <int NT, typename T>
@@ -964,7 +1016,12 @@ __device__ __forceinline__ int sample_from_list(const FilterLaunch& p, int r, co
         for (int c = threadIdx.x; c < f.chunks; c += NT) sm.list.hit[c] = c;
         __syncthreads();
     } else if (expect > fminf(0.9f * kListCap, 64.0f + 0.125f * (float)row.vocab)) {
-        return kNeedBins;  // too many for the list, or more to sort than the row is to read again
+        // too many for the list, or more to sort than the row is to read again
+        if (NT != 1024 || !open || f.chunks < 2 * kFewChunks || !(span > 0.0f) || !(span < 1e37f)) return kNeedBins;
+        const float part = use_p ? rule.topp : rule.coin;
+        cut = cut_by_number<NT>(f.chunks, f.top, f.low_chunk, f.z, part * f.sum, sm);
+        if (!(cut >= f.low_chunk)) return kNeedBins;
+        hits = (int)sm.hits;
     }
     const bool complete = !(cut > -inf);
     const int per = 2 + f.chunk_shift, items = hits << per;  // kU << chunk_shift vectors a chunk, one a thread
@@ -1339,8 +1396,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) filtered_sample_kernel(FilterLa
 template <typename T>
 void launch_rows(const FilterLaunch& p, int num_sms, cudaStream_t stream) {
     // Measured (1 B200): 4096 x 32000 fp32, top-p of Zipf rows: 225 us, of which pass 1,
-    // all of the HBM traffic, 105; 1 x 32000 15 us; 64 x 128000 bf16 21 us, and 103
-    // when one of its rows has to take the bins (about 1 peaked row in 2000 does).
+    // all of the HBM traffic, 105; 1 x 32000 15 us; 64 x 128000 bf16 21 us.
     // Threads of a row.  Up to two rows an SM: enough of them that a warp has a batch
     // or two, for the row's latency.  More rows: several on an SM at a time, whose
     // passes overlap; a row of at most 16 batches leaves 8 warps too little between

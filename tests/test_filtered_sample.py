@@ -407,3 +407,33 @@ def test_reference_walk_on_known_rows():
     assert reference_row(x, 1.0, 0, 0.5, 0.0, 0.9)[:3:2] == (2, 1)
     assert reference_row(x, 1.0, 0, 1.0, 0.4, 0.9)[:3:2] == (1, 2)
     assert reference_row(x, 0.0, 0, 1.0, 0.0, 0.9)[:3:2] == (2, 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [32000, 128000])
+def test_heavy_entries_side_by_side(pkg, dtype, V):
+    """Most of the mass in a few entries that lie next to one another, above a broad floor: the
+    largest of a stretch says little of its mass.  Row by row another number of them, up to rows
+    in which they hold just less than top-p asks for."""
+    g = torch.Generator().manual_seed(V)
+    x = torch.randn(12, V, generator=g) * 2.2
+    for b in range(12):
+        x[b, 4096:4096 + 8] = torch.linspace(18.0, 15.0 - 0.25 * b, 8)
+        x[b, 9000 + 700 * b: 9000 + 700 * b + 3] = 16.0
+    x = x.to(dtype).cuda()
+    for p in (0.5, 0.9, 0.95, 0.99):
+        check(pkg, x, 0.8, 0, p, 0.0, coins_of(12, 31))
+        check(pkg, x, 1.0, 0, p, 0.0, coins_of(12, 32))
+    check(pkg, x, 0.8, 0, 1.0, 0.0, coins_of(12, 33))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_rows_of_equal_logits(pkg, dtype):
+    """All weights 1, so every border is exact: ids and counts follow from integers."""
+    for V in (31, 1000, 32001):
+        x = torch.full((4, V), 2.5, dtype=dtype).cuda()
+        x[3, V // 2] = float("nan")
+        for rule in ("open", "topp", "all"):
+            check(pkg, x, *RULES[rule], coins_of(4, V))

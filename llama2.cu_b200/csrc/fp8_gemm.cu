@@ -26,7 +26,7 @@
 // What bounds it: for large batches the way of a TMEM buffer from its last product
 // to its next first one (commit, loads, release, issue: some 650 ns, of which the
 // other buffer's product covers 520), for small ones the stream of W.
-// Measured (1 B200): 8192 x 4096 x 32000 1.17 ms in a short run, 1.45 in a long one
+// Measured (1 B200): 8192 x 4096 x 32000 1.23 ms in a short run, 1.45 in a long one
 // under the power cap (0.92 with one accumulation over all of K, which the scales do
 // not allow); 1 x 4096 x 32000 28 us, of which 20 are the bytes.
 // Every mbarrier wait is bounded; a timeout sets the error word and drains

@@ -548,12 +548,20 @@ enum { kDone = 0, kNeedSum64 = 1, kNeedBins = 2, kNeedExact = 3 };
 
 // Pass 1: maximum, chunk maxima and mass; with kLow the minimum too (an open
 // row with -infinity among its entries has to count its candidates).  A chunk is
-// what one lane reads of 2^chunk_shift batches.  Weights are 2^(x * z - R) with
-// an integer R, z in two words: two FMAs with one rounding each, and a new R (when
-// a weight would pass 2^60) rescales by a power of two, exactly.  So a weight is
-// off by 2 * 2^-25 * ln 2 * |log2 w| relative and ex2's 2^-22, the trees by 5
-// steps; the mean of |log2 w| under the weights is H - log2 S <= log2(V / S) bits.
-// Sums of trees are fp64.
+// what one lane reads of 2^chunk_shift batches.  Weights are 2^t, t = x * z - R with
+// an integer R and z in two words: two FMAs, each off by 2^-24 |t| at most.  R is a
+// warp's own, the rounded exponent of the largest logit when it was set, and is set
+// again (which rescales the sum by a power of two, exactly) as soon as t would pass
+// kRefBits.  So |t| is at most |log2 w| + kRefBits + 1 for a weight w against the row's top,
+// or against the warp's when that is lower, and the mean of |log2 w| under the weights is
+// H - log2 S <= log2(V / S).  Where x * z is large, z's first word puts R and the limit
+// off by 2^-22 |x * z| each.  The sum of the weights is thus off by
+//   2^-24 * (2 ln 2 * (log2(V / S) + kRefBits + 1 + 2^-20 |top * z|) + 4 + 5 + 1)
+// relative at most: the arguments, ex2 (2^-22), the trees (5 levels) and the result.
+// Sums of trees are fp64.  An R that lags by more than a few bits is what the bound
+// cannot have: at 40 octaves, each argument's rounding is 2^-19 of its weight.
+constexpr float kRefBits = 4.0f;
+
 template <int NT, typename T, bool kLow>
 __device__ __forceinline__ void first_pass(const VecRow<T>& row, int shift, uint4 (&raw)[kU], FastSmem<NT>& sm,
                                            RowFacts& f) {
@@ -596,7 +604,7 @@ __device__ __forceinline__ void first_pass(const VecRow<T>& row, int shift, uint
             const float r = rintf(warp_max(m) * z_hi), d = ref - r;
             run_sum *= limit > -inf && d > -126.0f ? (double)__int_as_float((127 + (int)d) << 23) : 0.0;
             ref = r;
-            limit = (r + 60.0f) / z_hi;
+            limit = (r + kRefBits) / z_hi;
         }
         const u64 rr = pack2(-ref, -ref);
         u64 t[kU];
@@ -647,8 +655,8 @@ __device__ __forceinline__ void first_pass(const VecRow<T>& row, int shift, uint
     for (int o = NW / 2; o; o >>= 1) s += __shfl_xor_sync(kFullMask, s, o);
     s = __shfl_sync(kFullMask, s, 0);
     f.sum = (float)(s * exp2_64((double)all - (double)top * f.z64));
-    const float bits = fmaxf(__log2f((float)row.vocab / f.sum), 0.0f) + 1.0f;
-    f.sum_err = 6e-8f * (0.7f * bits + 11.0f);  // units of 2^-24; the sum's own rounding and half a bit of R among them
+    const float bits = fmaxf(__log2f((float)row.vocab / f.sum), 0.0f) + kRefBits + 1.0f + 1e-6f * fabsf(all);
+    f.sum_err = 6e-8f * (1.39f * bits + 10.5f);  // 2^-24 and 2 ln 2, with room for second orders
     f.top = top;
     f.low = kLow ? low : -inf;
     f.low_chunk = low_chunk;
@@ -875,6 +883,7 @@ __device__ int decide_list(const FilterLaunch& p, int r, const RowRule& rule, co
     if (!listed && !use_p) {
         if (at >= n) return kNeedBins;
         if (count_below(cum, n, (double)rule.coin * hi) != at) return kNeedSum64;
+        if (p.logprobs && err > 0x1p-18 * sum) return kNeedSum64;  // logits far from 0 against T
         kept = candidates;
         lo = sum;
     }

@@ -1,0 +1,121 @@
+"""sample_filtered at the borders between two entries: coins and top-p values on
+either side of a running mass, close to it.  The definition is formed with 64-bit
+mantissas (numpy's long double), so that its own rounding, 2^-64 an operation, stays far
+below the distances tested.
+
+Ids and counts are compared exactly.  That is a demand on the kernel only where a
+border is farther away than the kernel's weights are off: 2^-43 of the largest
+weight each.  The coins of these rows are multiples of 2^-24, and `far_enough`
+leaves out those that lie closer than that to a border.
+"""
+import numpy as np
+import pytest
+import torch
+
+from test_filtered_sample import call
+
+LD = np.longdouble
+
+
+class Row:
+    """The order, running masses and mass of one row without NaN or infinities above."""
+
+    def __init__(self, x, T):
+        x = np.asarray(x, LD)
+        order = np.argsort(-x, kind="stable")
+        self.order = order[x[order] > -np.inf]
+        v = x[self.order]
+        with np.errstate(over="ignore", under="ignore"):
+            w = np.exp((v - v[0]) / LD(T))
+        self.cum = np.cumsum(w)
+        self.mass = self.cum[-1]
+
+    def far_enough(self, part, share=2.0 ** -43):
+        """part * mass is farther than `share` of the mass from every running mass."""
+        at = np.searchsorted(self.cum, LD(part) * self.mass)
+        near = self.cum[max(at - 1, 0):at + 2]
+        return bool((np.abs(near - LD(part) * self.mass) > LD(share) * self.mass).all())
+
+    def place(self, part):
+        """Entries whose running mass is at most part * mass."""
+        return int(np.searchsorted(self.cum, LD(part) * self.mass, side="right"))
+
+
+def heads_above_a_floor(V, first, T, bits, seed, n=20):
+    """Noise, and n entries some `bits` octaves of weight above it, at places from `first` on."""
+    g = np.random.default_rng(seed)
+    x = g.standard_normal(V)
+    at = g.choice(np.arange(first, V), n, replace=False)
+    x[at] = bits * np.log(2.0) * T + 0.6 * T * g.standard_normal(n)
+    return x.astype(np.float32)
+
+
+STEPS = (-24, -12, -6, -3, -1, 0, 1, 2, 4, 7, 13, 25)
+
+
+def coins_at_borders(row, lowest=0.2):
+    """Multiples of 2^-24 on either side of every border above `lowest`."""
+    out = []
+    for b in (row.cum / row.mass)[:40]:
+        if b < lowest or b > 1 - LD(2) ** -20:
+            continue
+        for s in STEPS:
+            c = (int(np.floor(b * 2 ** 24)) + s) / 2.0 ** 24
+            if 0 <= c < 1 and row.far_enough(c):
+                out.append(c)
+    return np.array(out, np.float32)
+
+
+def parts_at_borders(row, lowest=0.2):
+    """fp32 numbers on either side of every border above `lowest`."""
+    out = []
+    for b in (row.cum / row.mass)[:40]:
+        if b < lowest or b > 1 - LD(2) ** -20:
+            continue
+        near = np.float32(b)
+        for s in STEPS:
+            c = np.float32(near + s * np.spacing(near))
+            if 0 < c < 1 and row.far_enough(c):
+                out.append(c)
+    return np.array(out, np.float32)
+
+
+def check_borders(pkg, xs, T, dtype=torch.float32, most=4096, bits=None):
+    """Every row of xs once for each coin, and once for each top-p value, at its borders, in calls of at most `most` rows."""
+    logits, coins, ids, parts, kept = [], [], [], [], []
+    xs = torch.from_numpy(np.stack(xs)).to(dtype)
+    for i, x in enumerate(xs.float().numpy()):
+        row = Row(x, np.float32(T))
+        c, p = coins_at_borders(row), parts_at_borders(row)
+        coins.append(c)
+        parts.append(p)
+        ids.append([row.order[row.place(v)] for v in c])
+        kept.append([row.place(v) + 1 for v in p])
+    for which, values, want in (("coin", coins, ids), ("top-p", parts, kept)):
+        of = torch.from_numpy(np.repeat(np.arange(len(xs)), [len(v) for v in values]))
+        values, want = np.concatenate(values), np.concatenate(want)
+        assert len(values) > 0
+        for lo in range(0, len(values), most):
+            part = slice(lo, lo + most)
+            logits = xs[of[part]].cuda()
+            if which == "coin":
+                got = call(pkg, logits, T, 0, 1.0, 0.0, values[part])[0]
+            else:
+                got = call(pkg, logits, T, 0, values[part], 0.0, np.zeros(len(values[part]), np.float32))[2]
+            bad = np.nonzero(got != want[part])[0]
+            assert len(bad) == 0, (f"{which}: {len(bad)} of {len(got)} rows, the first at {values[part][bad[0]]!r}: "
+                                   f"{got[bad[0]]}, not {want[part][bad[0]]}")
+
+
+# V and rows a call: 1024 threads a row, 256 and 128
+FORMS = [(32000, 256), (32000, 4096), (8000, 4096)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [0.5, 0.6, 0.7, 0.8])
+@pytest.mark.parametrize("V,most", FORMS)
+def test_borders_of_entries_far_above_their_warps_first(pkg, V, most, T):
+    """The heads lie where each warp has read a batch of the floor before, 30 to 55 octaves below them."""
+    first = 16384 if most < 297 else 4096
+    xs = [heads_above_a_floor(V, first, T, bits, 100 * i + bits) for i in range(2) for bits in (30, 41, 55)]
+    check_borders(pkg, xs, T, most=most)

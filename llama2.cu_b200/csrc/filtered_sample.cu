@@ -541,6 +541,8 @@ struct RowFacts {
     float minp_at;     // logits of at least this pass min-p (-infinity when off)
     int chunks;
     int chunk_shift;   // log2 of the batches of a chunk
+    // the difference first, which fp64 holds: x * z - top * z would round the second product,
+    // by 2^-38 of the weight at top / T = 30000
     __device__ __forceinline__ double weight(float x) const { return exp2_64(((double)x - (double)top) * z64); }
 };
 
@@ -664,17 +666,16 @@ __device__ __forceinline__ void first_pass(const VecRow<T>& row, int shift, uint
     f.chunks = ((row.batches + group) >> shift) << 5;
 }
 
-// The mass in fp64 of the whole row.
+// The mass in fp64 of the whole row, of weights as the lists have them.
 template <int NT, typename T>
 __device__ __noinline__ double sum64(const VecRow<T>& row, const RowFacts& f, FastSmem<NT>& sm) {
     constexpr int E = VecRow<T>::E;
-    const double c = -(double)f.top * f.z64;
     double s = 0.0;
     for (int vec = threadIdx.x; vec < row.vecs; vec += NT) {
         float v[E];
         VecRow<T>::widen(row.load(vec), v);
 #pragma unroll
-        for (int e = 0; e < E; ++e) s += exp2_64(fma((double)v[e], f.z64, c));
+        for (int e = 0; e < E; ++e) s += f.weight(v[e]);
     }
     return block_sum<NT>(s, sm.red_d);
 }
@@ -1159,7 +1160,6 @@ __device__ __forceinline__ double gather_brackets(const VecRow<T>& row, const Ro
                                                   int last, int split, Bracket (&br)[2], FastSmem<NT>& sm) {
     constexpr int E = VecRow<T>::E;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const double c = -(double)f.top * f.z64;
     if (threadIdx.x < 2) sm.n[threadIdx.x] = 0u;
     __syncthreads();
     double all = 0.0, mass[2] = {0.0, 0.0};
@@ -1187,7 +1187,7 @@ __device__ __forceinline__ double gather_brackets(const VecRow<T>& row, const Ro
                 mask0 |= (in && !a0 && at < br[0].hi) ? 1u << e : 0u;
                 mask1 |= (in && !a1 && at < br[1].hi) ? 1u << e : 0u;
                 if (kMass) {
-                    const double m = in ? exp2_64(fma((double)v[e], f.z64, c)) : 0.0;
+                    const double m = in ? f.weight(v[e]) : 0.0;
                     all += m;
                     mass[0] += a0 ? m : 0.0;
                     mass[1] += a1 ? m : 0.0;

@@ -119,3 +119,63 @@ def test_borders_of_entries_far_above_their_warps_first(pkg, V, most, T):
     first = 16384 if most < 297 else 4096
     xs = [heads_above_a_floor(V, first, T, bits, 100 * i + bits) for i in range(2) for bits in (30, 41, 55)]
     check_borders(pkg, xs, T, most=most)
+
+
+def close_coin(rows, T, lowest, highest):
+    """Of rows of logits, the ones with a coin that lies between `lowest` and `highest` of the mass from a border of
+    its row; [(row, coin, id)]."""
+    out = []
+    for x in rows:
+        row = Row(x, np.float32(T))
+        share = row.cum / row.mass
+        near = np.rint(share * 2 ** 24)
+        away = np.abs(near / LD(2) ** 24 - share)
+        for i in np.nonzero((away > lowest) & (away < highest) & (near > 0) & (near < 2 ** 24))[0]:
+            c = float(near[i]) / 2.0 ** 24
+            out.append((x, c, row.order[row.place(c)]))
+    return out
+
+
+def check_close(pkg, cases, T, dtype=torch.float32):
+    x = torch.from_numpy(np.stack([c[0] for c in cases])).to(dtype).cuda()
+    got = call(pkg, x, T, 0, 1.0, 0.0, np.array([c[1] for c in cases], np.float32))[0]
+    bad = np.nonzero(got != np.array([c[2] for c in cases]))[0]
+    assert len(bad) == 0, f"{len(bad)} of {len(got)} rows"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,top", [(1e-3, 60.3), (1e-3, -35.7), (1e-4, 20.6), (1e-2, 1500.3)])
+def test_borders_far_from_zero_against_the_temperature(pkg, T, top):
+    """Two or three entries share the mass, top / T is 3.5e4 to 2e5, and the coin is 2^-43 to 2^-39 of the mass off a
+    border: fp32 sums leave it open, and what settles it has to hold the weights to 2^-43."""
+    g = np.random.default_rng(int(abs(top)))
+    base = (top - 100.0 + np.abs(g.standard_normal(2000))).astype(np.float32)
+    step = abs(float(np.spacing(np.float32(top))))
+    reach = max(int(2.0 * T / step), 40)
+    heads = []
+    want = LD(2) ** 24
+    while len(heads) < 24:  # the first border is 1 / S of the mass: it has to fall next to a multiple of 2^-24
+        near = np.float32(top) - step * g.integers(1, reach, (200000, 3)).astype(np.float64)
+        w = np.exp((near.astype(np.float32).astype(LD) - LD(np.float32(top))) / LD(np.float32(T))).sum(1) + 1
+        share = 1 / w
+        away = np.abs(np.rint(share * want) / want - share)
+        heads += [near[i] for i in np.nonzero((away > LD(2) ** -42.5) & (away < LD(2) ** -39))[0]]
+    rows = []
+    for h in heads[:24]:
+        x = base.copy()
+        x[[100, 700, 1300, 1900]] = np.concatenate([[top], h])
+        rows.append(x)
+    cases = close_coin(rows, T, LD(2) ** -42.5, LD(2) ** -39)
+    assert len(cases) >= 24
+    check_close(pkg, cases, T)
+
+
+@pytest.mark.gpu
+def test_borders_of_flat_rows_far_from_zero(pkg):
+    """The same where no list holds the mass: a row of 32000 near 60 at T = 0.001 has a coin within 2^-40 of a border or
+    two."""
+    g = np.random.default_rng(5)
+    rows = [(60.3 + 0.002 * g.standard_normal(32000)).astype(np.float32) for _ in range(24)]
+    cases = close_coin(rows, 1e-3, LD(2) ** -42.5, LD(2) ** -39)
+    assert len(cases) >= 24
+    check_close(pkg, cases, 1e-3)

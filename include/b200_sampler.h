@@ -307,7 +307,8 @@ typedef struct {
 /* Samples `batch` rows by temperature, top-k, top-p and min-p with one random
  * number per row.  The entries of a row above -infinity are its candidates,
  * ordered by falling logit, ties by rising index; entry i has the weight
- * w_i = exp((l_i - max l) / T), and the filters keep a prefix of the order:
+ * w_i = exp((l_i - max l) / T), at T = +infinity 1 where l_i and max l are
+ * finite, and the filters keep a prefix of the order:
  *   n1 = the candidates, of these the first topk, of these those with w_i >= minp
  *   n  = the shortest prefix whose mass exceeds topp * (mass of the n1), or n1
  * The token is the first of the n whose running mass exceeds

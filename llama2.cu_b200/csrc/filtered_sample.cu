@@ -75,7 +75,7 @@ __device__ __forceinline__ RowRule row_rule(const FilterLaunch& p, int row, bool
     RowRule r;
     const float t = p.temperature_rows ? p.temperature_rows[row] : p.temperature;
     r.greedy = !(t >= kGreedyBelow);
-    r.temperature = fminf(t, 3.402823466e38f);  // so that -infinity / T stays one
+    r.temperature = t;
     r.topk = p.topk_rows ? p.topk_rows[row] : p.topk;
     r.topp = p.topp_rows ? p.topp_rows[row] : p.topp;
     r.minp = p.minp_rows ? p.minp_rows[row] : p.minp;
@@ -92,6 +92,10 @@ __device__ __forceinline__ RowRule row_rule(const FilterLaunch& p, int row, bool
     r.coin = fminf(fmaxf(c, 0.0f), 0x1.fffffep-1f);  // NaN counts as 0
     return r;
 }
+
+// The temperature in fp64.  Infinity counts as a number that no difference of two
+// logits comes near: finite logits weigh the same, and -infinity nothing.
+__device__ __forceinline__ double temperature64(float t) { return t > 3.402823466e38f ? 1e300 : (double)t; }
 
 // exp((x - top) / T); 1 at the top whatever its value is.
 __device__ __forceinline__ double weight64(float x, float top, double T) {
@@ -254,7 +258,7 @@ __device__ __noinline__ void sample_exact(const FilterLaunch& p, int r, RowRule 
         return;
     }
     row.top = key_value(top_key);
-    row.temperature = rule.greedy ? 1.0 : (double)rule.temperature;
+    row.temperature = rule.greedy ? 1.0 : temperature64(rule.temperature);
     u64 n = n0, total = 0;
     // mass and count of everything, and of what min-p keeps
     const bool use_minp = rule.minp > 0.0f && !rule.greedy;
@@ -572,7 +576,9 @@ __device__ __forceinline__ void first_pass(const VecRow<T>& row, int shift, uint
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const float inf = __int_as_float(0x7F800000);
     const float z_hi = __double2float_rd(f.z64);
-    const float z_lo = fmaxf(__double2float_rd(f.z64 - (double)z_hi), 1e-37f);  // above 0: -infinity stays itself
+    // above 0, for -infinity to stay itself: the smallest number there is, as z itself is that small
+    // where T is that large
+    const float z_lo = fmaxf(__double2float_rd(f.z64 - (double)z_hi), 0x1p-149f);
     const int group = (1 << shift) - 1;
     const u64 zz_hi = pack2(z_hi, z_hi), zz_lo = pack2(z_lo, z_lo);
     float ref = 0.0f, limit = -inf, top = -inf, chunk = -inf, low = inf, low_chunk = inf;
@@ -659,6 +665,8 @@ __device__ __forceinline__ void first_pass(const VecRow<T>& row, int shift, uint
     f.sum = (float)(s * exp2_64((double)all - (double)top * f.z64));
     const float bits = fmaxf(__log2f((float)row.vocab / f.sum), 0.0f) + kRefBits + 1.0f + 1e-6f * fabsf(all);
     f.sum_err = 6e-8f * (1.39f * bits + 10.5f);  // 2^-24 and 2 ln 2, with room for second orders
+    // where z's second word is a subnormal number it is off by up to 2^-149, times logits 2^129 apart
+    f.sum_err += f.z < 0x1p-100f ? 7e-7f : 0.0f;
     f.top = top;
     f.low = kLow ? low : -inf;
     f.low_chunk = low_chunk;
@@ -1378,7 +1386,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) filtered_sample_kernel(FilterLa
         sm.n[0] = 0u;
     }
     RowFacts f;
-    f.z64 = rule.greedy ? 1.0 : 1.4426950408889634074 / (double)rule.temperature;
+    f.z64 = rule.greedy ? 1.0 : 1.4426950408889634074 / temperature64(rule.temperature);
     f.z = (float)f.z64;
     const int k = rule.topk > 0 && rule.topk < p.vocab ? rule.topk : 0;
     const bool open = !rule.greedy && k == 0 && !(rule.minp > 0.0f) && !(rule.topp > 0.0f && rule.topp < 1.0f);
@@ -1392,9 +1400,11 @@ __global__ void __launch_bounds__(NT, 1024 / NT) filtered_sample_kernel(FilterLa
         return;
     }
     if (plain && f.sum > 0.0f && f.sum < 1e30f) {
-        f.minp_at = rule.minp > 0.0f
-                        ? __double2float_ru((double)f.top + (double)rule.temperature * log(fmin((double)rule.minp, 1.0)))
-                        : -__int_as_float(0x7F800000);
+        f.minp_at = -__int_as_float(0x7F800000);
+        if (rule.minp > 0.0f) {
+            const double at = (double)f.top + temperature64(rule.temperature) * log(fmin((double)rule.minp, 1.0));
+            f.minp_at = rule.temperature > 3.402823466e38f ? kLowest : __double2float_ru(at);
+        }
         st = sample_from_list<NT>(p, r, row, rule, f, k, sm);
         if (st == kNeedBins) st = sample_by_bins<NT>(p, r, row, rule, f, k, sm);
     }

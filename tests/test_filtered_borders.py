@@ -12,7 +12,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_filtered_sample import call
+from test_filtered_sample import call, check
 
 LD = np.longdouble
 
@@ -179,3 +179,40 @@ def test_borders_of_flat_rows_far_from_zero(pkg):
     cases = close_coin(rows, 1e-3, LD(2) ** -42.5, LD(2) ** -39)
     assert len(cases) >= 24
     check_close(pkg, cases, 1e-3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T", [1e5, 1e30, 2e36, 1e37, 1.2e38, 3e38, float("inf")])
+def test_large_temperatures_over_the_whole_range_of_logits(pkg, dtype, T):
+    """Temperatures at which logits of the type's lowest value have a share; all finite logits have the same at infinity."""
+    low = float(torch.finfo(dtype).min)
+    for V in (2000, 40000):
+        g = torch.Generator().manual_seed(V)
+        x = torch.full((7, V), low)
+        x[0, V // 3] = 0.0
+        x[1] = torch.rand(V, generator=g) * low
+        x[2, ::2] = torch.randn(V // 2, generator=g)
+        x[3, V // 2:] = -float("inf")
+        x[4] = (2.0 * torch.rand(V, generator=g) - 1.0) * (-low)
+        x[5, ::3] = -float("inf")
+        x[5, 1] = 30.0
+        x[6] = torch.randn(V, generator=g)
+        x = x.to(dtype).cuda()
+        for k, p, q in ((0, 1.0, 0.0), (0, 0.9, 0.0), (0, 0.3, 0.0), (0, 1.0, 0.4), (50, 1.0, 0.0), (700, 0.8, 0.1)):
+            for c in (0.0, 0.25, 0.5, 0.7531, 1.0):
+                check(pkg, x, T, k, p, q, np.full(7, c, np.float32))
+
+
+@pytest.mark.gpu
+def test_infinite_logits_and_temperature(pkg):
+    """Entries of +infinity share the whole mass at every temperature, an infinite one included."""
+    x = torch.randn(4, 3000)
+    x[:, [5, 77, 2000]] = float("inf")
+    x[2, 9] = float("nan")
+    x[3, 100:200] = -float("inf")
+    got = call(pkg, x.cuda(), float("inf"), 0, 1.0, 0.0, np.array([0.1, 0.5, 0.9, 0.999], np.float32))
+    assert got[0].tolist() == [5, 77, 2000, 2000]
+    assert np.allclose(got[1], -np.log(3.0), rtol=0, atol=2.0 ** -17)
+    got = call(pkg, x.cuda(), float("inf"), 0, 1.0, 0.5, np.zeros(4, np.float32))
+    assert got[2].tolist() == [3] * 4

@@ -581,7 +581,9 @@ __device__ __forceinline__ void first_pass(const VecRow<T>& row, int shift, uint
     const float z_lo = fmaxf(__double2float_rd(f.z64 - (double)z_hi), 0x1p-149f);
     const int group = (1 << shift) - 1;
     const u64 zz_hi = pack2(z_hi, z_hi), zz_lo = pack2(z_lo, z_lo);
-    float ref = 0.0f, limit = -inf, top = -inf, chunk = -inf, low = inf, low_chunk = inf;
+    // R starts as the smallest there is: entries that x * z takes below it (a mask of the type's lowest
+    // value at a T below 1.4) weigh nothing, and must not make R infinite and the weights NaN
+    float ref = -3e38f, limit = -inf, top = -inf, chunk = -inf, low = inf, low_chunk = inf;
     double run_sum = 0.0;
     int b = warp << shift;
     while (b < row.batches) {
@@ -609,8 +611,8 @@ __device__ __forceinline__ void first_pass(const VecRow<T>& row, int shift, uint
             chunk = -inf;
         }
         if (__any_sync(kFullMask, m > limit)) {
-            const float r = rintf(warp_max(m) * z_hi), d = ref - r;
-            run_sum *= limit > -inf && d > -126.0f ? (double)__int_as_float((127 + (int)d) << 23) : 0.0;
+            const float r = fmaxf(rintf(warp_max(m) * z_hi), ref), d = ref - r;
+            run_sum *= d > -126.0f ? (double)__int_as_float((127 + (int)d) << 23) : 0.0;
             ref = r;
             limit = (r + kRefBits) / z_hi;
         }

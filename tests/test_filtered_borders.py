@@ -216,3 +216,42 @@ def test_infinite_logits_and_temperature(pkg):
     assert np.allclose(got[1], -np.log(3.0), rtol=0, atol=2.0 ** -17)
     got = call(pkg, x.cuda(), float("inf"), 0, 1.0, 0.5, np.zeros(4, np.float32))
     assert got[2].tolist() == [3] * 4
+
+
+def time_of(pkg, x, rule, coins):
+    """Microseconds of a call, the least of several runs of ten."""
+    ids = torch.empty(x.shape[0], dtype=torch.int32, device="cuda")
+    best = float("inf")
+    for _ in range(8):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        torch.cuda.synchronize()
+        a.record()
+        for _ in range(10):
+            pkg.sample_filtered(x, *rule, coins=coins, out_ids=ids)
+        b.record()
+        torch.cuda.synchronize()
+        best = min(best, a.elapsed_time(b) * 100)
+    return best
+
+
+MASKS = {"first half": slice(0, 16000), "a third": slice(10000, 20000), "padding": slice(31800, 32000)}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mask", sorted(MASKS))
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rule", [(0.8, 0, 1.0, 0.05)])
+def test_masks_of_the_lowest_value_do_not_take_the_radix_path(pkg, rule, dtype, mask):
+    """A masked stretch of the row, by the type's lowest value and by -infinity: the same ids, and no more than three
+    times the time (the radix path takes 8 to 20 times as long)."""
+    x = torch.from_numpy(np.stack([heads_above_a_floor(32000, 0, 1.0, 14, s) for s in range(4)]))
+    coins = np.array([0.1, 0.4, 0.6, 0.95], np.float32)
+    c = torch.from_numpy(coins).cuda()
+    times = []
+    for value in (-float("inf"), float(torch.finfo(dtype).min)):
+        y = x.clone()
+        y[:, MASKS[mask]] = value
+        y = y.to(dtype).cuda()
+        check(pkg, y, *rule, coins)
+        times.append(time_of(pkg, y, rule, c))
+    assert times[1] <= 3.0 * times[0], times

@@ -22,7 +22,8 @@
 //      fp64 sums above the brackets and the entries inside them (sample_by_bins)
 // Pass 1's fp32 sum decides only what its error bound allows; else the row is
 // summed again in fp64.  What fits neither (NaN, infinities, more entries in a
-// bracket than its list holds, as with equal logits) takes sample_exact: a radix descent over the
+// bracket than its list holds, as with equal logits, a top-k larger than the number
+// of chunks that hold more than a finite mask) takes sample_exact: a radix descent over the
 // 32-bit ordered keys with masses in fp64 summed as 64-bit integers in units
 // of 2^-43, in which equal keys are resolved by division.
 // Ids are thus those of real arithmetic up to about 2^-43 of the largest
@@ -324,6 +325,7 @@ constexpr int kChunkBins = 512;    // bins of the chunk maxima
 constexpr int kChunkCap = 2048;    // chunk maxima kept: 64 groups of batches, one a lane
 constexpr int kU = 4;              // vectors of a lane in a batch
 constexpr int kFewChunks = 192;    // chunks of the second try of pass 2
+constexpr int kCoarse = 16;        // bins that are too few for a threshold with many chunks above it
 constexpr int kShortList = 128;    // a list of up to this many is put in order by counting
 constexpr float kLowest = -3.402823466e38f;
 
@@ -954,11 +956,63 @@ __device__ __noinline__ float cut_by_number(int chunks, float top, float low_chu
     return all >= 0.75 * (double)mass && sm.hits <= 2 * kFewChunks ? cut : __int_as_float(0x7FC00000);
 }
 
+// The threshold of pass 2 once more, with bins over the chunk maxima from `coarse` on
+// only, and the chunks above it listed again: for rows whose range is stretched far below what
+// matters, as by logits masked with a large negative number, so that one bin holds all the
+// others (32000 fp32, top-k 50, half of them at the lowest value: 243 us by the radix path that a
+// list too long ends in, 20 so).  Leaves the smallest of these maxima in sm.red_f[2][0].
+template <int NT>
+__device__ __noinline__ float finer_cut(int chunks, float top, float z, float coarse, bool by_count, float want,
+                                        FastSmem<NT>& sm) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const float inf = __int_as_float(0x7F800000);
+    float low = inf;
+    for (int i = threadIdx.x; i < chunks; i += NT)
+        if (sm.chunk_max[i] >= coarse) low = fminf(low, sm.chunk_max[i]);
+    low = warp_min(low);
+    __syncthreads();
+    if (lane == 0) sm.red_f[2][warp] = low;
+    for (int i = threadIdx.x; i < kChunkBins; i += NT) sm.chunk_bin[i] = 0u;
+    if (threadIdx.x == 0) sm.hits = 0u;
+    __syncthreads();
+    low = warp_min(sm.red_f[2][lane < NT / 32 ? lane : 0]);
+    const float scale = top > low ? (float)(kChunkBins - 1) / (top - low) : 0.0f;
+    for (int i = threadIdx.x; i < chunks; i += NT) {
+        const float m = sm.chunk_max[i];
+        if (m >= low)
+            atomicAdd(&sm.chunk_bin[min((int)((top - m) * scale), kChunkBins - 1)],
+                      by_count ? 1u : (unsigned)(ex2_approx((m - top) * z) * 0x1p20f));
+    }
+    __syncthreads();
+    constexpr int R = kChunkBins / 32;  // every warp forms the same threshold
+    unsigned c = 0;
+    for (int j = 0; j < R; ++j) c += sm.chunk_bin[lane * R + j];
+    unsigned ci = c;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned cu = __shfl_up_sync(kFullMask, ci, o);
+        if (lane >= o) ci += cu;
+    }
+    ci -= c;
+    int found = kChunkBins;
+    for (int j = 0; j < R; ++j) {
+        ci += sm.chunk_bin[lane * R + j];
+        if ((float)ci >= want && found == kChunkBins) found = lane * R + j;
+    }
+    found = __reduce_min_sync(kFullMask, found);
+    const float cut = found < kChunkBins && top > low ? fmaxf(__fsub_rd(top, ((float)found + 1.01f) / scale), coarse) : low;
+    for (int i = threadIdx.x; i < chunks; i += NT)
+        if (sm.chunk_max[i] >= cut) sm.list.hit[atomicAdd(&sm.hits, 1u)] = i;
+    if (threadIdx.x == 0) sm.red_f[2][0] = low;
+    __syncthreads();
+    return cut;
+}
+
 // Pass 2: a threshold below which nothing can be kept or drawn, and the row
 // decided by the list of the entries above it.
 template <int NT, typename T>
 __device__ __forceinline__ int sample_from_list(const FilterLaunch& p, int r, const VecRow<T>& row, const RowRule& rule,
-                                                const RowFacts& f, int k, FastSmem<NT>& sm) {
+                                                RowFacts& f, int k, FastSmem<NT>& sm) {
     constexpr int E = VecRow<T>::E;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const float inf = __int_as_float(0x7F800000);
@@ -968,7 +1022,7 @@ __device__ __forceinline__ int sample_from_list(const FilterLaunch& p, int r, co
     // chunk maxima over [low_chunk, top]: how many, and how much mass in them alone,
     // lie at or above each bin's lower edge.  Bin b is at 32 * (b % 16) + b / 16, so
     // that the lanes of the scan, 16 bins each, read 32 banks.
-    const float span = f.top - f.low_chunk;
+    float span = f.top - f.low_chunk;
     const float scale = span > 0.0f ? (float)(kChunkBins - 1) / span : 0.0f;
     if (open || k > 0) {
         for (int i = threadIdx.x; i < f.chunks; i += NT) {
@@ -982,7 +1036,8 @@ __device__ __forceinline__ int sample_from_list(const FilterLaunch& p, int r, co
         __syncthreads();
     }
     // every warp forms the same threshold
-    float cut = -inf;
+    float cut = -inf, want = 0.0f;
+    int found = kChunkBins;
     if (open || k > 0) {
         constexpr int R = kChunkBins / 32;
         unsigned v[R], c = 0;
@@ -998,8 +1053,7 @@ __device__ __forceinline__ int sample_from_list(const FilterLaunch& p, int r, co
         // the first bin by which the chunk maxima alone hold k entries, or the mass asked for
         // (each is rounded down to 2^-20 of the largest; decide_list sees to the rest)
         const float part = use_p ? rule.topp : rule.coin;
-        const float want = k > 0 ? (float)k : part * f.sum * 1.00001f * 0x1p20f;
-        int found = kChunkBins;
+        want = k > 0 ? (float)k : part * f.sum * 1.00001f * 0x1p20f;
 #pragma unroll
         for (int j = 0; j < R; ++j) {
             ci += v[j];
@@ -1026,6 +1080,12 @@ __device__ __forceinline__ int sample_from_list(const FilterLaunch& p, int r, co
     }
     __syncthreads();
     int hits = (int)sm.hits;
+    if (found < kCoarse && hits > kFewChunks) {
+        cut = finer_cut<NT>(f.chunks, f.top, f.z, fmaxf(cut, kLowest), k > 0, want, sm);
+        hits = (int)sm.hits;
+        f.low_chunk = sm.red_f[2][0];
+        span = f.top - f.low_chunk;
+    }
     // entries to expect, were they spread over the chunks at random
     const float g = (float)f.chunks;
     const float expect = hits < f.chunks ? -g * __logf(1.0f - (float)hits / g) : 1e9f;

@@ -250,6 +250,11 @@ int sampler_gather_rows(const float* table, int table_rows, int dim, const int* 
  * device stays usable; later calls run normally.  polls in [1, 2^24]. */
 int sampler_selftest_wait_timeout(unsigned polls, int* row_flag);
 
+/* The same of classifier_fp8_sample_filtered: two rows whose products are never
+ * issued, so that the wait for them runs out after `polls` polls.  Allocates and
+ * frees device memory. */
+int classifier_fp8_selftest_wait_timeout(unsigned polls, int* row_flag);
+
 /* Largest vocabulary sampler_batched_noalloc accepts. */
 #define SAMPLER_NOALLOC_MAX_VOCAB 32768
 
@@ -363,7 +368,9 @@ int rmsnorm_fp8(const void* x, int x_dtype, const float* norm_weight, int batch,
  *   logits_out              [batch, ld], SAMPLER_DTYPE_F32 or _BF16, ld >= vocab (what lies between the
  *                           rows stays as it is)
  * dim % 16 == 0, dim <= 65536; hidden and wcls 16-byte aligned; any vocab.  The product of two scales
- * has to be a finite fp32 number. */
+ * has to be a finite fp32 number.  Logits that a device wait that ran out leaves unfinished are NaN; as
+ * the call does not synchronize, the next synchronizing call on the device reports it
+ * (SAMPLER_E_DEVICE). */
 int classifier_logits_fp8(const void* hidden, const float* hidden_scales, const void* wcls, const float* wcls_scales,
                           int batch, int dim, int vocab, void* logits_out, int logits_dtype, long long ld,
                           void* stream);
@@ -380,7 +387,9 @@ size_t classifier_fp8_workspace_bytes(int batch, int dim, int vocab, int logits_
  *   workspace   a device buffer of classifier_fp8_workspace_bytes(), 16-byte
  *               aligned, for the 8-bit operand and the logits; the caller's, so
  *               that calls which may overlap, and graphs whose replays may, have
- *               one each */
+ *               one each
+ * A row some of whose logits a device wait that ran out left unfinished gets id 0, 0
+ * kept entries, log probability -infinity and SAMPLER_ROW_TIMEOUT in row_flags. */
 int classifier_fp8_sample_filtered(const SamplerFilterConfig* cfg, const void* x, int x_dtype,
                                    const float* norm_weight, const void* wcls, const float* wcls_scales, int batch,
                                    int dim, const float* temperature_rows, const int* topk_rows,

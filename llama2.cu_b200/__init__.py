@@ -31,7 +31,7 @@ EXPORTED_SYMBOLS = [
     "sampler_nccl_comm_destroy", "sampler_batched_noalloc", "classifier_sample_fused",
     "classifier_logits", "rmsnorm_bf16", "classifier_rmsnorm_sample_fused", "sampler_gather_rows",
     "sampler_selftest_wait_timeout", "sampler_filtered", "quantize_fp8", "rmsnorm_fp8", "classifier_logits_fp8",
-    "classifier_fp8_workspace_bytes", "classifier_fp8_sample_filtered",
+    "classifier_fp8_workspace_bytes", "classifier_fp8_sample_filtered", "classifier_fp8_selftest_wait_timeout",
 ]
 
 
@@ -134,6 +134,8 @@ def lib():
     L.sampler_gather_rows.restype = c_int
     L.sampler_selftest_wait_timeout.argtypes = [ctypes.c_uint, ctypes.POINTER(c_int)]
     L.sampler_selftest_wait_timeout.restype = c_int
+    L.classifier_fp8_selftest_wait_timeout.argtypes = [ctypes.c_uint, ctypes.POINTER(c_int)]
+    L.classifier_fp8_selftest_wait_timeout.restype = c_int
     c_ll = ctypes.c_longlong
     L.sampler_filtered.argtypes = [ctypes.POINTER(SamplerFilterConfig), P, c_int, c_ll, P, P, P, P, P, P, P, P, P, P, P]
     L.sampler_filtered.restype = c_int

@@ -121,6 +121,11 @@ struct ExactSmem {
     int id;
 };
 
+// Whether the 8-bit product left this logit out (its own NaN, of the two types it writes).
+__device__ __forceinline__ bool unfinished(float x) { return __float_as_uint(x) == kUnfinishedF32; }
+__device__ __forceinline__ bool unfinished(__nv_bfloat16 x) { return __bfloat16_as_ushort(x) == kUnfinishedBf16; }
+__device__ __forceinline__ bool unfinished(__half) { return false; }
+
 // One row, element by element from global memory.
 template <typename T>
 struct RowView {
@@ -233,11 +238,12 @@ __device__ __noinline__ void sample_exact(const FilterLaunch& p, int r, RowRule 
     }
     __syncthreads();
     unsigned top_key = 0, candidates = 0;
-    bool nan = false;
+    bool nan = false, lost = false;
     for (int i = threadIdx.x; i < p.vocab; i += NT) {
         const float v = row.value(i);
         const unsigned k = order_key(v);
         nan |= v != v;
+        lost |= unfinished(row.x[i]);
         top_key = max(top_key, k);
         candidates += k != 0u;
     }
@@ -246,14 +252,15 @@ __device__ __noinline__ void sample_exact(const FilterLaunch& p, int r, RowRule 
     const int any_nan = __syncthreads_or(nan);
     top_key = sm.red_key;
     const u64 n0 = sm.red_count;
+    const bool timeout = p.from_product && __syncthreads_or(lost);
     __syncthreads();
     int flags = any_nan ? kFlagNan : 0;
-    if (n0 == 0) {
+    if (n0 == 0 || timeout) {  // of a row whose logits are not all there, nothing is used
         if (threadIdx.x == 0) {
             p.out_ids[r] = 0;
             if (p.logprobs) p.logprobs[r] = __int_as_float(0xFF800000);
             if (p.kept) p.kept[r] = 0;
-            if (p.row_flags) p.row_flags[r] = flags | kFlagNoCand;
+            if (p.row_flags) p.row_flags[r] = timeout ? kFlagTimeout : flags | kFlagNoCand;
         }
         __syncthreads();
         return;

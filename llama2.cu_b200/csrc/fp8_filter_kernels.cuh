@@ -10,6 +10,11 @@ namespace b2s {
 // Element types of the 16- and 32-bit inputs (mirrors of the public SAMPLER_DTYPE_* values).
 constexpr int kDtypeF32 = 0, kDtypeBf16 = 1, kDtypeF16 = 2;
 
+// What the product writes for a logit that it did not finish because a device wait ran
+// out: a NaN of a payload that no arithmetic has (instructions give 0x7FFFFFFF and 0x7FFF).
+constexpr uint32_t kUnfinishedF32 = 0xFFC0BAD0u;
+constexpr uint16_t kUnfinishedBf16 = 0xFFDAu;
+
 // float8 e4m3 values and fp32 scales of blocks of 128 columns (fp8_quant.cu).
 struct QuantLaunch {
     const void* x;             // [rows, ld], dtype
@@ -37,6 +42,7 @@ struct Fp8GemmLaunch {
     int out_bf16;
     long long ld;
     int* error_word;
+    unsigned wait_test;     // self-test: no products are issued, waits run out after so many polls; else 0
     int box_rows;           // set by the launch: rows of H that a tile loads
     int vec_out;            // set by the launch: rows of logits start on 16-byte boundaries
 };
@@ -45,6 +51,7 @@ struct Fp8GemmLaunch {
 struct FilterLaunch {
     const void* logits;  // [batch, ld], dtype
     int dtype;
+    int from_product;    // the logits are the 8-bit product's, which marks what it did not finish
     long long ld;
     int batch;
     int vocab;

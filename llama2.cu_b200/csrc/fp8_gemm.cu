@@ -29,8 +29,8 @@
 // Measured (1 B200): 8192 x 4096 x 32000 1.23 ms in a short run, 1.45 in a long one
 // under the power cap (0.92 with one accumulation over all of K, which the scales do
 // not allow); 1 x 4096 x 32000 28 us, of which 20 are the bytes.
-// Every mbarrier wait is bounded; a timeout sets the error word and drains
-// the pipeline.
+// Every mbarrier wait is bounded; a timeout sets the error word, fills the rest of the
+// CTA's tiles with a NaN of its own and drains the pipeline.
 #include "device_common.cuh"
 #include "fp8_filter_kernels.cuh"
 #include "tcgen05_common.cuh"
@@ -127,8 +127,9 @@ __device__ __forceinline__ float2 halves_of(unsigned long long v) {
 __device__ __forceinline__ bool fp8_aborted(const Fp8Smem& sm) { return *(const volatile int*)&sm.abort != 0; }
 // Bounded wait, inline: one thread issues all products and one all copies, and
 // every instruction of their loops is on a block's way.
-__device__ __forceinline__ bool fp8_wait(unsigned long long* bar, unsigned parity, Fp8Smem& sm, int* error_word) {
-    for (unsigned i = 0; i < kSpinLimit; ++i)
+__device__ __forceinline__ bool fp8_wait(unsigned long long* bar, unsigned parity, Fp8Smem& sm, int* error_word,
+                                         unsigned limit) {
+    for (unsigned i = 0; i < limit; ++i)
         if (mbar_try_wait(bar, parity)) return true;
     sm.abort = 1;
     atomicOr(error_word, 2);
@@ -196,7 +197,8 @@ __device__ __forceinline__ void fp8_tile_coords(int tile, int mt, int nt, int& m
 // its TMEM columns hold and writes NC - 128): a loop of its own for it cost a
 // quarter of the rate, in instruction fetches.
 template <int NC>
-__device__ __forceinline__ void fold_tiles(const Fp8GemmLaunch& p, Fp8Smem& sm, uint32_t tmem, int mt, int nt, int nk) {
+__device__ __forceinline__ void fold_tiles(const Fp8GemmLaunch& p, Fp8Smem& sm, uint32_t tmem, int mt, int nt, int nk,
+                                           unsigned limit) {
     constexpr bool kAligned = NC % kFK == 0;  // the columns lie in one block of 128 rows of W
     constexpr int kCols = kFCols;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q = warp & 3;
@@ -205,14 +207,15 @@ __device__ __forceinline__ void fold_tiles(const Fp8GemmLaunch& p, Fp8Smem& sm, 
     const int wblocks = (p.vocab + kFK - 1) / kFK;
     unsigned it = 0;
     bool ok = true;
-    for (int tile = blockIdx.x; tile < ntiles && ok; tile += gridDim.x) {
+    int tile = blockIdx.x;
+    for (; tile < ntiles && ok; tile += gridDim.x) {
         int mb, nb;
         fp8_tile_coords(tile, mt, nt, mb, nb);
         const int row0 = mb * kFM + q * 32, row = row0 + lane;
         const int wcol = nb * NC + col0;
         if (NC < kFN && row0 >= p.batch) {  // no rows of H here: the buffers are given back unread
             for (int k = 0; k < nk; ++k, ++it) {
-                ok = ok && fp8_wait(&sm.tmem_full[it & 1u], it >> 1 & 1u, sm, p.error_word);
+                ok = ok && fp8_wait(&sm.tmem_full[it & 1u], it >> 1 & 1u, sm, p.error_word, limit);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sm.tmem_empty[it & 1u]);
             }
@@ -241,7 +244,7 @@ __device__ __forceinline__ void fold_tiles(const Fp8GemmLaunch& p, Fp8Smem& sm, 
             // After a wait that ran out the rest of the tile is folded without waiting (and not
             // written): nothing but the wait stands between a buffer's arrival and its loads (a
             // look at the abort word here cost a quarter of the rate).
-            ok = ok && fp8_wait(&sm.tmem_full[buf], it >> 1 & 1u, sm, p.error_word);
+            ok = ok && fp8_wait(&sm.tmem_full[buf], it >> 1 & 1u, sm, p.error_word, limit);
             __syncwarp();
             tc_fence_after();
             const uint32_t src = tmem + ((uint32_t)(q * 32) << 16) + buf * kFN + (uint32_t)col0;
@@ -311,9 +314,23 @@ __device__ __forceinline__ void fold_tiles(const Fp8GemmLaunch& p, Fp8Smem& sm, 
             }
         }
     }
+    if (!ok)  // this tile and those behind it
+        for (; tile < ntiles; tile += gridDim.x) {
+            int mb, nb;
+            fp8_tile_coords(tile, mt, nt, mb, nb);
+            const int row = mb * kFM + q * 32 + lane, wcol = nb * NC + col0;
+            if (row >= p.batch) continue;
+            const long long at = (long long)row * p.ld + wcol;
+            for (int c = min(NC - col0, p.vocab - wcol) - 1; c >= 0; --c) {
+                if (p.out_bf16) static_cast<uint16_t*>(p.logits)[at + c] = kUnfinishedBf16;
+                else static_cast<uint32_t*>(p.logits)[at + c] = kUnfinishedF32;
+            }
+        }
 }
 
-template <int NC>
+// kTest: the self-test's form, which issues no products, so that the fold warps' first
+// wait runs out on a barrier nothing arrives at.
+template <int NC, bool kTest>
 __global__ void __launch_bounds__(kFThreads, 1)
     fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_h, const __grid_constant__ CUtensorMap tmap_w,
                     Fp8GemmLaunch p) {
@@ -324,6 +341,7 @@ __global__ void __launch_bounds__(kFThreads, 1)
     const int nt = (p.vocab + NC - 1) / NC;
     const int ntiles = mt * nt;
     const int nk = (p.dim + kFK - 1) / kFK;
+    const unsigned limit = kTest ? p.wait_test : kSpinLimit;
 
     const auto load_stage = [&](unsigned stage, int k, int mb, int nb) {
         mbar_arrive_expect_tx(&sm.full[stage], (unsigned)(p.box_rows + NC) * kFK);
@@ -368,7 +386,7 @@ __global__ void __launch_bounds__(kFThreads, 1)
                 int mb, nb;
                 fp8_tile_coords(tile, mt, nt, mb, nb);
                 for (; k < nk; ++k) {
-                    if (!fp8_wait(&sm.empty[stage], phase ^ 1u, sm, p.error_word)) break;
+                    if (!fp8_wait(&sm.empty[stage], phase ^ 1u, sm, p.error_word, limit)) break;
                     load_stage(stage, k, mb, nb);
                     if (++stage == kFStages) {
                         stage = 0;
@@ -376,9 +394,12 @@ __global__ void __launch_bounds__(kFThreads, 1)
                     }
                 }
             }
-            // drain: every stage this thread filled completes before the CTA exits
+            // drain: every copy this thread issued has landed before the CTA exits, whether or not
+            // products still took it (from `stage` on, a stage's last fill is of the pass before) ..
+            for (unsigned s = 0; s < kFStages; ++s) mbar_wait_bounded(&sm.full[s], s < stage ? phase : phase ^ 1u);
+            // .. and every stage it filled has been given back, if products went on
             for (int s = 0; s < kFStages; ++s) {
-                if (!mbar_wait_bounded(&sm.empty[stage], phase ^ 1u)) break;
+                if (!mbar_wait_bounded(&sm.empty[stage], phase ^ 1u, limit)) break;
                 if (++stage == kFStages) {
                     stage = 0;
                     phase ^= 1u;
@@ -392,12 +413,12 @@ __global__ void __launch_bounds__(kFThreads, 1)
             constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(NC >> 3) << 17) | ((uint32_t)(kFM >> 4) << 24);
             const uint64_t da0 = smem_desc_sw128(smem_addr(sm.a[0])), db0 = smem_desc_sw128(smem_addr(sm.b[0]));
             unsigned stage = 0, phase = 0, it = 0;
-            bool ok = true;
+            bool ok = !kTest;
             for (int tile = blockIdx.x; tile < ntiles && ok && !fp8_aborted(sm); tile += gridDim.x) {
                 for (int k = 0; k < nk; ++k, ++it) {
                     const unsigned buf = it & 1u, turn = it >> 1 & 1u;
-                    if (!fp8_wait(&sm.tmem_empty[buf], turn ^ 1u, sm, p.error_word) ||
-                        !fp8_wait(&sm.full[stage], phase, sm, p.error_word)) {
+                    if (!fp8_wait(&sm.tmem_empty[buf], turn ^ 1u, sm, p.error_word, limit) ||
+                        !fp8_wait(&sm.full[stage], phase, sm, p.error_word, limit)) {
                         ok = false;
                         break;
                     }
@@ -421,7 +442,7 @@ __global__ void __launch_bounds__(kFThreads, 1)
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         // ---- fold: warp w reads TMEM lanes 32 * (w % 4) .. +31
-        if (NC > kFCols || warp < 8) fold_tiles<NC>(p, sm, tmem, mt, nt, nk);
+        if (NC > kFCols || warp < 8) fold_tiles<NC>(p, sm, tmem, mt, nt, nk, limit);
     }
     tc_fence_before();
     __syncthreads();
@@ -444,7 +465,7 @@ bool make_tmap_fp8(CUtensorMap* m, const void* base, int rows, int dim, int box_
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int NC>
+template <int NC, bool kTest = false>
 cudaError_t launch_fp8(const Fp8GemmLaunch& p, int num_sms, cudaStream_t stream) {
     CUtensorMap th, tw;
     if (!make_tmap_fp8(&th, p.h, p.batch, p.dim, p.box_rows) || !make_tmap_fp8(&tw, p.w, p.vocab, p.dim, NC))
@@ -455,13 +476,14 @@ cudaError_t launch_fp8(const Fp8GemmLaunch& p, int num_sms, cudaStream_t stream)
     static std::atomic<unsigned long long> attr_done{0};
     const unsigned long long bit = 1ull << (dev & 63);
     if (!(attr_done.load() & bit)) {
-        e = cudaFuncSetAttribute(fp8_gemm_kernel<NC>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kFp8SmemBytes);
+        e = cudaFuncSetAttribute(fp8_gemm_kernel<NC, kTest>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 (int)kFp8SmemBytes);
         if (e != cudaSuccess) return e;
         attr_done.fetch_or(bit);
     }
     const long long tiles = (long long)((p.batch + kFM - 1) / kFM) * ((p.vocab + NC - 1) / NC);
     const int grid = tiles < num_sms ? (int)tiles : num_sms;
-    fp8_gemm_kernel<NC><<<grid, kFThreads, kFp8SmemBytes, stream>>>(th, tw, p);
+    fp8_gemm_kernel<NC, kTest><<<grid, kFThreads, kFp8SmemBytes, stream>>>(th, tw, p);
     return cudaGetLastError();
 }
 
@@ -485,7 +507,8 @@ int launch_fp8_gemm(const Fp8GemmLaunch& args, int num_sms, cudaStream_t stream)
         }
     }
     cudaError_t e;
-    if (cols == 256) e = launch_fp8<256>(p, num_sms, stream);
+    if (p.wait_test) e = launch_fp8<kFCols, true>(p, num_sms, stream);
+    else if (cols == 256) e = launch_fp8<256>(p, num_sms, stream);
     else if (cols == 224) e = launch_fp8<224>(p, num_sms, stream);
     else if (cols == 192) e = launch_fp8<192>(p, num_sms, stream);
     else if (cols == 160) e = launch_fp8<160>(p, num_sms, stream);

@@ -766,65 +766,10 @@ int quantize_call(const void* x, int x_dtype, const float* norm_weight, int rows
     g_last_launches = n;
     return SAMPLER_OK;
 }
-}  // namespace
 
-extern "C" {
-
-int sampler_filtered(const SamplerFilterConfig* cfg, const void* logits, int batch, long long ld,
-                     const float* temperature_rows, const int* topk_rows, const float* topp_rows,
-                     const float* minp_rows, const float* coins, unsigned long long* rng_state, int* out_ids,
-                     float* out_logprobs, int* out_kept, int* row_flags, void* stream) {
-    g_last_launches = 0;
-    int rc = check_filter_args(cfg, batch, temperature_rows, coins, rng_state, out_ids);
-    if (rc) return rc;
-    if (!logits || ld < cfg->vocab_size)
-        return fail(SAMPLER_E_INVALID, "null logits, or ld %lld below vocab %d", ld, cfg->vocab_size);
-    if ((uintptr_t)logits & (dtype_size(cfg->logits_dtype) - 1))
-        return fail(SAMPLER_E_INVALID, "logits not aligned to its elements");
-    if (batch == 0) return SAMPLER_OK;
-    DeviceCtx* c = nullptr;
-    rc = get_ctx(&c);
-    if (rc) return rc;
-    b2s::FilterLaunch f{};
-    f.logits = logits;
-    f.dtype = cfg->logits_dtype;
-    f.ld = ld;
-    f.batch = batch;
-    f.vocab = cfg->vocab_size;
-    f.temperature = cfg->temperature;
-    f.topk = cfg->topk;
-    f.topp = cfg->topp;
-    f.minp = cfg->minp;
-    f.temperature_rows = temperature_rows;
-    f.topk_rows = topk_rows;
-    f.topp_rows = topp_rows;
-    f.minp_rows = minp_rows;
-    f.coins = coins;
-    f.rng_state = rng_state;
-    f.out_ids = out_ids;
-    f.logprobs = out_logprobs;
-    f.kept = out_kept;
-    f.row_flags = row_flags;
-    const int n = b2s::launch_filtered_sample(f, c->num_sms, (cudaStream_t)stream);
-    if (n < 0) return fail(SAMPLER_E_CUDA, "filtered sampler launch: %s", cudaGetErrorString((cudaError_t)(-n)));
-    g_last_launches = n;
-    return SAMPLER_OK;
-}
-
-int quantize_fp8(const void* x, int x_dtype, int rows, int dim, long long ld, int block_rows, void* out_q,
-                 float* out_scales, void* stream) {
-    return quantize_call(x, x_dtype, nullptr, rows, dim, ld, block_rows, out_q, out_scales, (cudaStream_t)stream);
-}
-
-int rmsnorm_fp8(const void* x, int x_dtype, const float* norm_weight, int batch, int dim, long long ld, void* out_q,
-                float* out_scales, void* stream) {
-    if (!norm_weight) return fail(SAMPLER_E_INVALID, "null norm_weight");
-    return quantize_call(x, x_dtype, norm_weight, batch, dim, ld, 1, out_q, out_scales, (cudaStream_t)stream);
-}
-
-int classifier_logits_fp8(const void* hidden, const float* hidden_scales, const void* wcls, const float* wcls_scales,
-                          int batch, int dim, int vocab, void* logits_out, int logits_dtype, long long ld,
-                          void* stream) {
+int logits_fp8_call(const void* hidden, const float* hidden_scales, const void* wcls, const float* wcls_scales, int batch,
+                    int dim, int vocab, void* logits_out, int logits_dtype, long long ld, unsigned wait_test,
+                    cudaStream_t stream) {
     g_last_launches = 0;
     if (!hidden || !hidden_scales || !wcls || !wcls_scales || !logits_out)
         return fail(SAMPLER_E_INVALID, "null hidden, wcls, scales or logits_out");
@@ -857,26 +802,61 @@ int classifier_logits_fp8(const void* hidden, const float* hidden_scales, const 
     g.out_bf16 = logits_dtype == SAMPLER_DTYPE_BF16 ? 1 : 0;
     g.ld = ld;
     g.error_word = c->error_word;
-    const int n = b2s::launch_fp8_gemm(g, c->num_sms, (cudaStream_t)stream);
+    g.wait_test = wait_test;
+    const int n = b2s::launch_fp8_gemm(g, c->num_sms, stream);
     if (n < 0) return fail(SAMPLER_E_CUDA, "8-bit classifier launch: %s", cudaGetErrorString((cudaError_t)(-n)));
     g_last_launches = n;
     return SAMPLER_OK;
 }
 
-size_t classifier_fp8_workspace_bytes(int batch, int dim, int vocab, int logits_dtype) {
-    if (batch < 1 || dim < 1 || vocab < 1) return 0;
-    const size_t blocks = ((size_t)dim + 127) / 128;
-    const size_t operand = pad256((size_t)batch * dim) + pad256((size_t)batch * blocks * sizeof(float));
-    return operand + (logits_dtype < 0 ? 0 : (size_t)batch * vocab * dtype_size(logits_dtype));
+int filtered_call(const SamplerFilterConfig* cfg, const void* logits, int batch, long long ld,
+                  const float* temperature_rows, const int* topk_rows, const float* topp_rows,
+                  const float* minp_rows, const float* coins, unsigned long long* rng_state, int* out_ids,
+                  float* out_logprobs, int* out_kept, int* row_flags, bool from_product,
+                  cudaStream_t stream) {
+    g_last_launches = 0;
+    int rc = check_filter_args(cfg, batch, temperature_rows, coins, rng_state, out_ids);
+    if (rc) return rc;
+    if (!logits || ld < cfg->vocab_size)
+        return fail(SAMPLER_E_INVALID, "null logits, or ld %lld below vocab %d", ld, cfg->vocab_size);
+    if ((uintptr_t)logits & (dtype_size(cfg->logits_dtype) - 1))
+        return fail(SAMPLER_E_INVALID, "logits not aligned to its elements");
+    if (batch == 0) return SAMPLER_OK;
+    DeviceCtx* c = nullptr;
+    rc = get_ctx(&c);
+    if (rc) return rc;
+    b2s::FilterLaunch f{};
+    f.logits = logits;
+    f.dtype = cfg->logits_dtype;
+    f.ld = ld;
+    f.batch = batch;
+    f.vocab = cfg->vocab_size;
+    f.temperature = cfg->temperature;
+    f.topk = cfg->topk;
+    f.topp = cfg->topp;
+    f.minp = cfg->minp;
+    f.temperature_rows = temperature_rows;
+    f.topk_rows = topk_rows;
+    f.topp_rows = topp_rows;
+    f.minp_rows = minp_rows;
+    f.coins = coins;
+    f.rng_state = rng_state;
+    f.out_ids = out_ids;
+    f.logprobs = out_logprobs;
+    f.kept = out_kept;
+    f.row_flags = row_flags;
+    f.from_product = from_product ? 1 : 0;
+    const int n = b2s::launch_filtered_sample(f, c->num_sms, stream);
+    if (n < 0) return fail(SAMPLER_E_CUDA, "filtered sampler launch: %s", cudaGetErrorString((cudaError_t)(-n)));
+    g_last_launches = n;
+    return SAMPLER_OK;
 }
 
-int classifier_fp8_sample_filtered(const SamplerFilterConfig* cfg, const void* x, int x_dtype,
-                                   const float* norm_weight, const void* wcls, const float* wcls_scales, int batch,
-                                   int dim, const float* temperature_rows, const int* topk_rows,
-                                   const float* topp_rows, const float* minp_rows, const float* coins,
-                                   unsigned long long* rng_state, int* out_ids, float* out_logprobs, int* out_kept,
-                                   void* logits_out, int* row_flags, void* workspace, size_t workspace_bytes,
-                                   void* stream) {
+int fp8_step_call(const SamplerFilterConfig* cfg, const void* x, int x_dtype, const float* norm_weight, const void* wcls,
+                  const float* wcls_scales, int batch, int dim, const float* temperature_rows, const int* topk_rows,
+                  const float* topp_rows, const float* minp_rows, const float* coins, unsigned long long* rng_state,
+                  int* out_ids, float* out_logprobs, int* out_kept, void* logits_out, int* row_flags, void* workspace,
+                  size_t workspace_bytes, unsigned wait_test, cudaStream_t stream) {
     g_last_launches = 0;
     int rc = check_filter_args(cfg, batch, temperature_rows, coins, rng_state, out_ids);
     if (rc) return rc;
@@ -900,16 +880,64 @@ int classifier_fp8_sample_filtered(const SamplerFilterConfig* cfg, const void* x
     char* hq = static_cast<char*>(workspace);
     float* hs = reinterpret_cast<float*>(hq + pad256((size_t)batch * dim));
     void* logits = logits_out ? logits_out : hq + classifier_fp8_workspace_bytes(batch, dim, V, -1);
-    rc = quantize_call(x, x_dtype, norm_weight, batch, dim, dim, 1, hq, hs, (cudaStream_t)stream);
+    rc = quantize_call(x, x_dtype, norm_weight, batch, dim, dim, 1, hq, hs, stream);
     if (rc) return rc;
     int launches = g_last_launches;
-    rc = classifier_logits_fp8(hq, hs, wcls, wcls_scales, batch, dim, V, logits, cfg->logits_dtype, V, stream);
+    rc = logits_fp8_call(hq, hs, wcls, wcls_scales, batch, dim, V, logits, cfg->logits_dtype, V, wait_test, stream);
     if (rc) return rc;
     launches += g_last_launches;
-    rc = sampler_filtered(cfg, logits, batch, V, temperature_rows, topk_rows, topp_rows, minp_rows, coins, rng_state,
-                          out_ids, out_logprobs, out_kept, row_flags, stream);
+    rc = filtered_call(cfg, logits, batch, V, temperature_rows, topk_rows, topp_rows, minp_rows, coins, rng_state,
+                       out_ids, out_logprobs, out_kept, row_flags, true, stream);
     g_last_launches += launches;
     return rc;
+}
+}  // namespace
+
+extern "C" {
+
+int sampler_filtered(const SamplerFilterConfig* cfg, const void* logits, int batch, long long ld,
+                     const float* temperature_rows, const int* topk_rows, const float* topp_rows,
+                     const float* minp_rows, const float* coins, unsigned long long* rng_state, int* out_ids,
+                     float* out_logprobs, int* out_kept, int* row_flags, void* stream) {
+    return filtered_call(cfg, logits, batch, ld, temperature_rows, topk_rows, topp_rows, minp_rows, coins, rng_state,
+                         out_ids, out_logprobs, out_kept, row_flags, false, (cudaStream_t)stream);
+}
+
+int quantize_fp8(const void* x, int x_dtype, int rows, int dim, long long ld, int block_rows, void* out_q,
+                 float* out_scales, void* stream) {
+    return quantize_call(x, x_dtype, nullptr, rows, dim, ld, block_rows, out_q, out_scales, (cudaStream_t)stream);
+}
+
+int rmsnorm_fp8(const void* x, int x_dtype, const float* norm_weight, int batch, int dim, long long ld, void* out_q,
+                float* out_scales, void* stream) {
+    if (!norm_weight) return fail(SAMPLER_E_INVALID, "null norm_weight");
+    return quantize_call(x, x_dtype, norm_weight, batch, dim, ld, 1, out_q, out_scales, (cudaStream_t)stream);
+}
+
+int classifier_logits_fp8(const void* hidden, const float* hidden_scales, const void* wcls, const float* wcls_scales,
+                          int batch, int dim, int vocab, void* logits_out, int logits_dtype, long long ld,
+                          void* stream) {
+    return logits_fp8_call(hidden, hidden_scales, wcls, wcls_scales, batch, dim, vocab, logits_out, logits_dtype, ld,
+                           0, (cudaStream_t)stream);
+}
+
+size_t classifier_fp8_workspace_bytes(int batch, int dim, int vocab, int logits_dtype) {
+    if (batch < 1 || dim < 1 || vocab < 1) return 0;
+    const size_t blocks = ((size_t)dim + 127) / 128;
+    const size_t operand = pad256((size_t)batch * dim) + pad256((size_t)batch * blocks * sizeof(float));
+    return operand + (logits_dtype < 0 ? 0 : (size_t)batch * vocab * dtype_size(logits_dtype));
+}
+
+int classifier_fp8_sample_filtered(const SamplerFilterConfig* cfg, const void* x, int x_dtype,
+                                   const float* norm_weight, const void* wcls, const float* wcls_scales, int batch,
+                                   int dim, const float* temperature_rows, const int* topk_rows,
+                                   const float* topp_rows, const float* minp_rows, const float* coins,
+                                   unsigned long long* rng_state, int* out_ids, float* out_logprobs, int* out_kept,
+                                   void* logits_out, int* row_flags, void* workspace, size_t workspace_bytes,
+                                   void* stream) {
+    return fp8_step_call(cfg, x, x_dtype, norm_weight, wcls, wcls_scales, batch, dim, temperature_rows, topk_rows,
+                         topp_rows, minp_rows, coins, rng_state, out_ids, out_logprobs, out_kept, logits_out, row_flags,
+                         workspace, workspace_bytes, 0, (cudaStream_t)stream);
 }
 
 int sampler_batched_host(const SamplerBatchConfig* cfg, const float* logits, int batch, long long ld,
@@ -1039,6 +1067,47 @@ int sampler_selftest_wait_timeout(unsigned polls, int* row_flag) {
     g_last_launches = n;
     B2S_CUDA(cudaMemcpyAsync(row_flag, d_flag, sizeof(int), cudaMemcpyDeviceToHost, s));
     B2S_CUDA(cudaStreamSynchronize(s));
+    return check_device_word(c);
+}
+
+// The same of the decode step on 8-bit weights: two zero rows through the three kernels, the product
+// in its self-test form.
+int classifier_fp8_selftest_wait_timeout(unsigned polls, int* row_flag) {
+    g_last_launches = 0;
+    if (polls == 0 || polls > (1u << 24) || !row_flag)
+        return fail(SAMPLER_E_INVALID, "polls must be in [1, 2^24] and row_flag non-NULL");
+    DeviceCtx* c = nullptr;
+    int rc = get_ctx(&c);
+    if (rc) return rc;
+    std::lock_guard<std::mutex> host_lock(c->host_mu);
+    constexpr int B = 2, D = 256, V = 300;
+    constexpr size_t x_bytes = B * D * sizeof(float), w_bytes = (size_t)V * D, s_bytes = 1024;
+    const size_t ws_bytes = classifier_fp8_workspace_bytes(B, D, V, SAMPLER_DTYPE_F32);
+    const size_t all = x_bytes + w_bytes + s_bytes + ws_bytes + 256;  // each part a multiple of 256 but the last
+    static_assert(x_bytes % 256 == 0 && w_bytes % 256 == 0, "aligned parts");
+    char* buf = nullptr;
+    B2S_CUDA(cudaMalloc(reinterpret_cast<void**>(&buf), all));
+    char* const w = buf + x_bytes;
+    char* const scales = w + w_bytes;
+    int* const ids = reinterpret_cast<int*>(scales + s_bytes);
+    char* const ws = scales + s_bytes + 256;
+    SamplerFilterConfig cfg{};
+    cfg.vocab_size = V;
+    cfg.logits_dtype = SAMPLER_DTYPE_F32;
+    int out[2 * B] = {-1, -1, -1, -1};  // ids, flags
+    cudaStream_t s = c->stream;
+    cudaError_t e = cudaMemsetAsync(buf, 0, all, s);
+    if (e == cudaSuccess)
+        rc = fp8_step_call(&cfg, buf, SAMPLER_DTYPE_F32, nullptr, w, reinterpret_cast<const float*>(scales), B, D, nullptr,
+                           nullptr, nullptr, nullptr, nullptr, nullptr, ids, nullptr, nullptr, nullptr, ids + B, ws, ws_bytes,
+                           polls, s);
+    if (e == cudaSuccess && rc == SAMPLER_OK) e = cudaMemcpyAsync(out, ids, sizeof(out), cudaMemcpyDeviceToHost, s);
+    const cudaError_t done = cudaStreamSynchronize(s);
+    if (e == cudaSuccess) e = done;
+    cudaFree(buf);
+    if (rc) return rc;
+    if (e != cudaSuccess) return fail(SAMPLER_E_CUDA, "decode step self-test: %s", cudaGetErrorString(e));
+    *row_flag = out[B] == out[B + 1] && out[0] == 0 && out[1] == 0 ? out[B] : -1;
     return check_device_word(c);
 }
 

@@ -1438,8 +1438,10 @@ __device__ __forceinline__ void take_first_max(const FilterLaunch& p, int r, con
     }
 }
 
+// p stays where the launch put it: by value, its address for the functions out of line
+// would be of a copy that every thread makes (4096 x 32000 top-p 227 -> 205 us without).
 template <int NT, typename T>
-__global__ void __launch_bounds__(NT, 1024 / NT) filtered_sample_kernel(FilterLaunch p) {
+__global__ void __launch_bounds__(NT, 1024 / NT) filtered_sample_kernel(const __grid_constant__ FilterLaunch p) {
     __shared__ FastSmem<NT> sm;
     const int r = blockIdx.x;
     const VecRow<T> row(static_cast<const T*>(p.logits) + (long long)r * p.ld, p.vocab);

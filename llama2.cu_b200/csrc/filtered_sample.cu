@@ -98,6 +98,15 @@ __device__ __forceinline__ RowRule row_rule(const FilterLaunch& p, int row, bool
 // logits comes near: finite logits weigh the same, and -infinity nothing.
 __device__ __forceinline__ double temperature64(float t) { return t > 3.402823466e38f ? 1e300 : (double)t; }
 
+// The smallest logit that passes min-p, in every path the same: of real weights, where a
+// weight rounded to 64 bits could be 1 below the top.
+__device__ __forceinline__ float minp_threshold(float top, float t, float minp) {
+    const float inf = __int_as_float(0x7F800000);
+    if (top == inf) return top;
+    if (t == inf) return -3.402823466e38f;
+    return __double2float_ru((double)top + (double)t * log(fmin((double)minp, 1.0)));
+}
+
 // exp((x - top) / T); 1 at the top whatever its value is.
 __device__ __forceinline__ double weight64(float x, float top, double T) {
     return x == top ? 1.0 : exp(((double)x - (double)top) / T);
@@ -270,7 +279,7 @@ __device__ __noinline__ void sample_exact(const FilterLaunch& p, int r, RowRule 
     u64 n = n0, total = 0;
     // mass and count of everything, and of what min-p keeps
     const bool use_minp = rule.minp > 0.0f && !rule.greedy;
-    const double minp = fmin((double)rule.minp, 1.0);
+    const float minp_at = use_minp ? minp_threshold(row.top, rule.temperature, rule.minp) : 0.0f;
     if (threadIdx.x == 0) sm.red_count = 0;
     __syncthreads();
     {
@@ -278,7 +287,7 @@ __device__ __noinline__ void sample_exact(const FilterLaunch& p, int r, RowRule 
         unsigned c = 0;
         for (int i = threadIdx.x; i < p.vocab; i += NT) {
             const float v = row.value(i);
-            if (order_key(v) != 0u && (!use_minp || weight64(v, row.top, row.temperature) >= minp)) {
+            if (order_key(v) != 0u && (!use_minp || v >= minp_at)) {
                 m += row.mass_of(v);
                 ++c;
             }
@@ -1471,11 +1480,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) filtered_sample_kernel(const __
         return;
     }
     if (plain && f.sum > 0.0f && f.sum < 1e30f) {
-        f.minp_at = -__int_as_float(0x7F800000);
-        if (rule.minp > 0.0f) {
-            const double at = (double)f.top + temperature64(rule.temperature) * log(fmin((double)rule.minp, 1.0));
-            f.minp_at = rule.temperature > 3.402823466e38f ? kLowest : __double2float_ru(at);
-        }
+        f.minp_at = rule.minp > 0.0f ? minp_threshold(f.top, rule.temperature, rule.minp) : -__int_as_float(0x7F800000);
         st = sample_from_list<NT>(p, r, row, rule, f, k, sm);
         if (st == kNeedBins) st = sample_by_bins<NT>(p, r, row, rule, f, k, sm);
     }

@@ -283,3 +283,21 @@ def test_finite_masks_of_every_extent(pkg, B, V):
                     check(pkg, y[rows].cuda(), 0.8, k, p, q, coins[rows])
                     for a, b in zip(got, few):
                         assert np.array_equal(a[rows], b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [0.7, 50.0, 1e20, 3e38, float("inf")])
+def test_min_p_is_the_same_with_and_without_a_nan(pkg, T):
+    """A NaN sends its row another way, on which the same entries pass min-p: those of real weights, of which 1 - 1e-19
+    is below a min-p of 1."""
+    g = np.random.default_rng(8)
+    V = 3000
+    x = torch.from_numpy(g.standard_normal((6, V)).astype(np.float32))
+    x[1, 40:90] = x[1].max()
+    y = torch.cat([x, torch.full((6, 1), float("nan"))], 1)
+    for q in (1.0, 0.999, 0.3, 7.0, 1e-30):
+        a = call(pkg, x.cuda(), T, 0, 1.0, q, np.full(6, 0.5, np.float32))
+        b = call(pkg, y.cuda(), T, 0, 1.0, q, np.full(6, 0.5, np.float32))
+        assert a[0].tolist() == b[0].tolist() and a[2].tolist() == b[2].tolist()
+        if T < 1e30 and q >= 1.0:
+            assert a[2].tolist() == (x == x.amax(1, keepdim=True)).sum(1).tolist()

@@ -334,9 +334,8 @@ typedef struct {
  *                    2^-17 relative; -infinity without candidates
  *   out_kept         [batch] or NULL: n
  *   row_flags        [batch] or NULL: SAMPLER_ROW_NAN, SAMPLER_ROW_NO_CANDIDATE
- * Weights and sums that decide an id are held to about 2^-43 of the largest
- * weight, so ids are those of real arithmetic up to that and do not depend on
- * scheduling.  With the same coin it draws as sampler_batched does when that
+ * What decides an id is held to about 2^-43 of the row's mass, so ids are those of
+ * real arithmetic up to that and do not depend on scheduling.  With the same coin it draws as sampler_batched does when that
  * row takes sample_topp; with top-p off, sampler_batched walks in index order
  * (sample_mult) and this call in falling order.  No workspace, no library
  * buffers: calls on different streams may overlap. */

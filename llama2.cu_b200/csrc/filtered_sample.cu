@@ -25,9 +25,9 @@
 // bracket than its list holds, as with equal logits, a top-k larger than the number
 // of chunks that hold more than a finite mask) takes sample_exact: a radix descent over the
 // 32-bit ordered keys with masses in fp64 summed as 64-bit integers in units
-// of 2^-43, in which equal keys are resolved by division.
-// Ids are thus those of real arithmetic up to about 2^-43 of the largest
-// weight, whatever the order of the sums was.
+// of 2^-62 to 2^-61 of the row's mass, in which equal keys are resolved by division.
+// Ids are thus those of real arithmetic up to about 2^-43 of the row's mass,
+// whatever the order of the sums was.
 #include "device_common.cuh"
 #include "fp8_filter_kernels.cuh"
 
@@ -42,7 +42,6 @@ namespace {
 typedef unsigned long long u64;
 
 constexpr int kFBins = 256;
-constexpr double kMassUnit = 8796093022208.0;  // 2^43: 2^20 entries of weight 1 fill 2^63
 constexpr float kGreedyBelow = 1e-6f;
 
 template <typename T>
@@ -142,9 +141,10 @@ struct RowView {
     int vocab;
     float top;
     double temperature;
+    double units;  // of mass in a weight of 1: a power of two, the row's mass is 2^61 to 2^62 of them
     __device__ __forceinline__ float value(int i) const { return as_f32<T>(x[i]); }
     __device__ __forceinline__ u64 mass_of(float v) const {
-        return (u64)__double2ll_rn(weight64(v, top, temperature) * kMassUnit);
+        return (u64)__double2ll_rn(weight64(v, top, temperature) * units);
     }
 };
 
@@ -162,7 +162,7 @@ __device__ Crossing find_crossing(const RowView<T>& row, u64 bound, ExactSmem& s
         }
         __syncthreads();
         // The lanes of one bin add together first: a row's leading digits are few, and
-        // those of a row of equal logits one.  A mass is at most 2^43: two words of 22
+        // those of a row of equal logits one.  A mass is at most 2^62: three words of 21
         // bits, whose sums over a warp fit 32.
         for (int base = 0; base < row.vocab; base += NT) {
             const int i = base + (int)threadIdx.x;
@@ -174,11 +174,12 @@ __device__ Crossing find_crossing(const RowView<T>& row, u64 bound, ExactSmem& s
             const unsigned group = __match_any_sync(kFullMask, bin);
             if (!in) continue;
             const u64 m = row.mass_of(v);
-            const unsigned lo = __reduce_add_sync(group, (unsigned)(m & 0x3FFFFFu));
-            const unsigned hi = __reduce_add_sync(group, (unsigned)(m >> 22));
+            const unsigned lo = __reduce_add_sync(group, (unsigned)m & 0x1FFFFFu);
+            const unsigned mid = __reduce_add_sync(group, (unsigned)(m >> 21) & 0x1FFFFFu);
+            const unsigned hi = __reduce_add_sync(group, (unsigned)(m >> 42));
             if ((int)(threadIdx.x & 31) == __ffs(group) - 1) {
                 atomicAdd(&sm.count[bin], (unsigned)__popc(group));
-                atomicAdd(&sm.mass[bin], ((u64)hi << 22) + lo);
+                atomicAdd(&sm.mass[bin], ((u64)hi << 42) + ((u64)mid << 21) + lo);
             }
         }
         __syncthreads();
@@ -233,8 +234,10 @@ __device__ int index_of_tie(const RowView<T>& row, uint32_t key, u64 rank, Exact
 }
 
 // The row by radix descents: right for every row, and slow (a row of 32000 fp32 by itself:
-// 0.47 ms with all logits equal, 0.32 with a NaN, 0.23 with an infinity; 15 us by the
-// list, 50 by the bins).
+// 0.48 ms with all logits equal, 0.37 with a NaN, 0.26 with an infinity; 14 us by the
+// list, 50 by the bins).  Masses are rounded to units of the row's mass: in units of 2^-43
+// of the largest weight, which needs two words and not three (0.32 with a NaN), 50000
+// roundings moved borders among the lightest entries.
 template <int NT, typename T>
 __device__ __noinline__ void sample_exact(const FilterLaunch& p, int r, RowRule rule, ExactSmem& sm) {
     RowView<T> row;
@@ -280,8 +283,25 @@ __device__ __noinline__ void sample_exact(const FilterLaunch& p, int r, RowRule 
     // mass and count of everything, and of what min-p keeps
     const bool use_minp = rule.minp > 0.0f && !rule.greedy;
     const float minp_at = use_minp ? minp_threshold(row.top, rule.temperature, rule.minp) : 0.0f;
-    if (threadIdx.x == 0) sm.red_count = 0;
-    __syncthreads();
+    {
+        // the mass in fp32, off by far less than 1%, which the units leave room for; the same in every call
+        // (a fixed order of sums)
+        __shared__ float part[NT / 32];
+        const float z = (float)(1.4426950408889634074 / row.temperature);
+        float s = 0.0f;
+        for (int i = threadIdx.x; i < p.vocab; i += NT) {
+            const float v = row.value(i);
+            if (order_key(v) != 0u) s += v == row.top ? 1.0f : ex2_approx(fmaxf(v - row.top, -3.402823466e38f) * z);
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(kFullMask, s, o);
+        if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
+        if (threadIdx.x == 0) sm.red_count = 0;
+        __syncthreads();
+        s = 0.0f;
+        for (int w = 0; w < NT / 32; ++w) s += part[w];
+        row.units = scalbn(1.0, 61 - ilogbf(1.01f * s));  // 1 <= s <= 2^20
+    }
     {
         u64 m = 0;
         unsigned c = 0;
@@ -323,7 +343,7 @@ __device__ __noinline__ void sample_exact(const FilterLaunch& p, int r, RowRule 
         p.out_ids[r] = id;
         if (p.logprobs) {
             const double d = key_value(c.key) == row.top ? 0.0 : ((double)key_value(c.key) - (double)row.top) / row.temperature;
-            p.logprobs[r] = (float)(d - log((double)total / kMassUnit));
+            p.logprobs[r] = (float)(d - log((double)total / row.units));
         }
         if (p.kept) p.kept[r] = (int)n;
         if (p.row_flags) p.row_flags[r] = flags;

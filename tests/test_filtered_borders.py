@@ -4,8 +4,8 @@ mantissas (numpy's long double), so that its own rounding, 2^-64 an operation, s
 below the distances tested.
 
 Ids and counts are compared exactly.  That is a demand on the kernel only where a
-border is farther away than the kernel's weights are off: 2^-43 of the largest
-weight each.  The coins of these rows are multiples of 2^-24, and `far_enough`
+border is farther away than the kernel's sums are off: 2^-43 of the row's mass.  The
+coins of these rows are multiples of 2^-24, and `far_enough`
 leaves out those that lie closer than that to a border.
 """
 import numpy as np
@@ -301,3 +301,29 @@ def test_min_p_is_the_same_with_and_without_a_nan(pkg, T):
         assert a[0].tolist() == b[0].tolist() and a[2].tolist() == b[2].tolist()
         if T < 1e30 and q >= 1.0:
             assert a[2].tolist() == (x == x.amax(1, keepdim=True)).sum(1).tolist()
+
+
+def rows_of_many_ties(n):
+    """Rows that take the radix path: fp16 logits around 100 in steps of 1/16, hundreds of equal ones at a crossing."""
+    g = np.random.default_rng(12)
+    return [torch.from_numpy(100.0 + 2.9 * g.standard_normal(57481)).half().float().numpy() for _ in range(n)]
+
+
+@pytest.mark.gpu
+def test_last_coins_over_many_ties(pkg):
+    """The largest coins fall among the lightest entries, each 2^-35 of the mass or less: sums in units that the largest
+    weight sets, not the mass, count 50000 roundings there."""
+    rows = rows_of_many_ties(16)
+    T = 0.75
+    logits, coins, ids = [], [], []
+    for x in rows:
+        row = Row(x, np.float32(T))
+        for j in range(1, 7):
+            c = 1.0 - j * 2.0 ** -24
+            if row.far_enough(c):
+                logits.append(x)
+                coins.append(c)
+                ids.append(row.order[row.place(c)])
+    assert len(ids) > 80
+    got = call(pkg, torch.from_numpy(np.stack(logits)).half().cuda(), T, 0, 1.0, 0.0, np.array(coins, np.float32))[0]
+    assert got.tolist() == ids

@@ -250,9 +250,9 @@ int sampler_gather_rows(const float* table, int table_rows, int dim, const int* 
  * device stays usable; later calls run normally.  polls in [1, 2^24]. */
 int sampler_selftest_wait_timeout(unsigned polls, int* row_flag);
 
-/* The same of classifier_fp8_sample_filtered: two rows whose products are never
- * issued, so that the wait for them runs out after `polls` polls.  Allocates and
- * frees device memory. */
+/* The same of classifier_fp8_sample_filtered, with logits of either type: two rows
+ * whose products are never issued, so that the wait for them runs out after `polls`
+ * polls; *row_flag is -1 if a row was not reported.  Allocates and frees device memory. */
 int classifier_fp8_selftest_wait_timeout(unsigned polls, int* row_flag);
 
 /* Largest vocabulary sampler_batched_noalloc accepts. */
@@ -355,7 +355,8 @@ int quantize_fp8(const void* x, int x_dtype, int rows, int dim, long long ld, in
                  float* out_scales, void* stream);
 
 /* The final RMSNorm (as rmsnorm_bf16, of rows in fp32 or 16 bits) and
- * quantize_fp8 of its fp32 result at block_rows 1, in one pass. */
+ * quantize_fp8 of its fp32 result at block_rows 1, in one pass.  The sum of squares is
+ * fp32 there and here: a row whose sum passes 3.4e38 comes out as zeros. */
 int rmsnorm_fp8(const void* x, int x_dtype, const float* norm_weight, int batch, int dim, long long ld, void* out_q,
                 float* out_scales, void* stream);
 

@@ -1071,7 +1071,7 @@ int sampler_selftest_wait_timeout(unsigned polls, int* row_flag) {
 }
 
 // The same of the decode step on 8-bit weights: two zero rows through the three kernels, the product
-// in its self-test form.
+// in its self-test form, with logits of either type.
 int classifier_fp8_selftest_wait_timeout(unsigned polls, int* row_flag) {
     g_last_launches = 0;
     if (polls == 0 || polls > (1u << 24) || !row_flag)
@@ -1093,21 +1093,26 @@ int classifier_fp8_selftest_wait_timeout(unsigned polls, int* row_flag) {
     char* const ws = scales + s_bytes + 256;
     SamplerFilterConfig cfg{};
     cfg.vocab_size = V;
-    cfg.logits_dtype = SAMPLER_DTYPE_F32;
     int out[2 * B] = {-1, -1, -1, -1};  // ids, flags
     cudaStream_t s = c->stream;
-    cudaError_t e = cudaMemsetAsync(buf, 0, all, s);
-    if (e == cudaSuccess)
-        rc = fp8_step_call(&cfg, buf, SAMPLER_DTYPE_F32, nullptr, w, reinterpret_cast<const float*>(scales), B, D, nullptr,
-                           nullptr, nullptr, nullptr, nullptr, nullptr, ids, nullptr, nullptr, nullptr, ids + B, ws, ws_bytes,
-                           polls, s);
-    if (e == cudaSuccess && rc == SAMPLER_OK) e = cudaMemcpyAsync(out, ids, sizeof(out), cudaMemcpyDeviceToHost, s);
-    const cudaError_t done = cudaStreamSynchronize(s);
-    if (e == cudaSuccess) e = done;
+    cudaError_t e = cudaSuccess;
+    bool all_flagged = true;
+    for (int type : {SAMPLER_DTYPE_F32, SAMPLER_DTYPE_BF16}) {
+        cfg.logits_dtype = type;
+        if (e == cudaSuccess) e = cudaMemsetAsync(buf, 0, all, s);
+        if (e == cudaSuccess && rc == SAMPLER_OK)
+            rc = fp8_step_call(&cfg, buf, SAMPLER_DTYPE_F32, nullptr, w, reinterpret_cast<const float*>(scales), B, D,
+                               nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, ids, nullptr, nullptr, nullptr,
+                               ids + B, ws, ws_bytes, polls, s);
+        if (e == cudaSuccess && rc == SAMPLER_OK) e = cudaMemcpyAsync(out, ids, sizeof(out), cudaMemcpyDeviceToHost, s);
+        const cudaError_t done = cudaStreamSynchronize(s);
+        if (e == cudaSuccess) e = done;
+        for (int b = 0; b < B; ++b) all_flagged = all_flagged && out[b] == 0 && out[B + b] == SAMPLER_ROW_TIMEOUT;
+    }
     cudaFree(buf);
     if (rc) return rc;
     if (e != cudaSuccess) return fail(SAMPLER_E_CUDA, "decode step self-test: %s", cudaGetErrorString(e));
-    *row_flag = out[B] == out[B + 1] && out[0] == 0 && out[1] == 0 ? out[B] : -1;
+    *row_flag = all_flagged ? SAMPLER_ROW_TIMEOUT : -1;
     return check_device_word(c);
 }
 

@@ -946,8 +946,8 @@ __device__ int decide_list(const FilterLaunch& p, int r, const RowRule& rule, co
 // entries far below them.  The kFewChunks largest maxima, if these nearly hold `mass`:
 // their chunks are listed and the threshold is returned, else NaN.  About 1 peaked
 // row in 1300 is such a one.  For the kernel of few rows, where one of them is the call's
-// time (64 x 128000 bf16, top-p: 104 us by the bins, 29 so); with many rows they hide
-// behind the others, and the tries of the rest cost more (4096 x 32000 222 -> 232 us).
+// time (64 x 128000 bf16, top-p: 102 us by the bins, 27 so); with many rows they hide
+// behind the others, and the tries of the rest cost more (4096 x 32000 206 -> 215 us).
 template <int NT>
 __device__ __noinline__ float cut_by_number(int chunks, float top, float low_chunk, float z, float mass,
                                             FastSmem<NT>& sm) {
@@ -995,8 +995,8 @@ __device__ __noinline__ float cut_by_number(int chunks, float top, float low_chu
 // The threshold of pass 2 once more, with bins over the chunk maxima from `coarse` on
 // only, and the chunks above it listed again: for rows whose range is stretched far below what
 // matters, as by logits masked with a large negative number, so that one bin holds all the
-// others (32000 fp32, top-k 50, half of them at the lowest value: 243 us by the radix path that a
-// list too long ends in, 20 so).  Leaves the smallest of these maxima in sm.red_f[2][0].
+// others (32000 fp32, top-k 50, half of them at the lowest value: 263 us by the radix path that a
+// list too long ends in, 21 so).  Leaves the smallest of these maxima in sm.red_f[2][0].
 template <int NT>
 __device__ __noinline__ float finer_cut(int chunks, float top, float z, float coarse, bool by_count, float want,
                                         FastSmem<NT>& sm) {
@@ -1036,7 +1036,8 @@ __device__ __noinline__ float finer_cut(int chunks, float top, float z, float co
         if ((float)ci >= want && found == kChunkBins) found = lane * R + j;
     }
     found = __reduce_min_sync(kFullMask, found);
-    const float cut = found < kChunkBins && top > low ? fmaxf(__fsub_rd(top, ((float)found + 1.01f) / scale), coarse) : low;
+    float cut = coarse;  // min-p's, or the rest's, where that leaves too few
+    if (found < kChunkBins) cut = top > low ? fmaxf(__fsub_rd(top, ((float)found + 1.01f) / scale), coarse) : low;
     for (int i = threadIdx.x; i < chunks; i += NT)
         if (sm.chunk_max[i] >= cut) sm.list.hit[atomicAdd(&sm.hits, 1u)] = i;
     if (threadIdx.x == 0) sm.red_f[2][0] = low;
@@ -1510,12 +1511,13 @@ __global__ void __launch_bounds__(NT, 1024 / NT) filtered_sample_kernel(const __
 
 template <typename T>
 void launch_rows(const FilterLaunch& p, int num_sms, cudaStream_t stream) {
-    // Measured (1 B200): 4096 x 32000 fp32, top-p of Zipf rows: 225 us, of which pass 1,
-    // all of the HBM traffic, 105; 1 x 32000 15 us; 64 x 128000 bf16 21 us.
+    // Measured (1 B200): 4096 x 32000 fp32, top-p of Zipf rows: 206 us, of which pass 1,
+    // all of the HBM traffic, 101; 1 x 32000 13 us; 64 x 128000 bf16 19 us (39 where a row's
+    // border is left open by pass 1 and its mass summed again).
     // Threads of a row.  Up to two rows an SM: enough of them that a warp has a batch
     // or two, for the row's latency.  More rows: several on an SM at a time, whose
     // passes overlap; a row of at most 16 batches leaves 8 warps too little between
-    // their barriers (4096 x 6000 bf16: 97 us with 8 warps, 68 with 4).
+    // their barriers (4096 x 6000 bf16: 73 us with 8 warps, 52 with 4).
     const long long batches = ((long long)p.vocab * sizeof(T) + 2047) / 2048;
     const bool few = p.batch <= 2 * num_sms;
     if (few && batches > 16) filtered_sample_kernel<1024, T><<<p.batch, 1024, 0, stream>>>(p);

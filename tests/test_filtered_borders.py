@@ -327,3 +327,20 @@ def test_last_coins_over_many_ties(pkg):
     assert len(ids) > 80
     got = call(pkg, torch.from_numpy(np.stack(logits)).half().cuda(), T, 0, 1.0, 0.0, np.array(coins, np.float32))[0]
     assert got.tolist() == ids
+
+
+@pytest.mark.gpu
+def test_finite_masks_with_top_k_and_min_p(pkg):
+    """Min-p leaves fewer than top-k asks for, above a masked half: the list of min-p's entries decides, as with
+    -infinity."""
+    x = torch.from_numpy(np.stack([heads_above_a_floor(32000, 0, 1.0, 14, s, n=300) for s in range(4)]))
+    coins = np.array([0.1, 0.4, 0.6, 0.95], np.float32)
+    c = torch.from_numpy(coins).cuda()
+    times = []
+    for value in (-float("inf"), float(np.finfo(np.float32).min)):
+        y = x.clone()
+        y[:, :16000] = value
+        y = y.cuda()
+        check(pkg, y, 0.8, 700, 1.0, 0.01, coins)
+        times.append(time_of(pkg, y, (0.8, 700, 1.0, 0.01), c))
+    assert times[1] <= 3.0 * times[0], times

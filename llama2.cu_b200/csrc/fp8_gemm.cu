@@ -25,10 +25,12 @@
 //
 // What bounds it: for large batches the way of a TMEM buffer from its last product
 // to its next first one (commit, loads, release, issue: some 650 ns, of which the
-// other buffer's product covers 520), for small ones the stream of W.
-// Measured (1 B200): 8192 x 4096 x 32000 1.23 ms in a short run, 1.45 in a long one
-// under the power cap (0.92 with one accumulation over all of K, which the scales do
-// not allow); 1 x 4096 x 32000 28 us, of which 20 are the bytes.
+// other buffer's product covers 520), for small ones two chains of about the same
+// length: the stream of W, and its blocks one after the other in each SM (32 of 520 to
+// 650 ns at 4096 wide), which the batch makes no longer.
+// Measured (1 B200): 8192 x 4096 x 32000 1.45 ms under the power cap, 1.23 in runs too
+// short to reach it (0.92 with one accumulation over all of K, which the scales do not
+// allow); 1 x 4096 x 32000 28 us, 31 with new inputs each time, of which 20 are the bytes.
 // Every mbarrier wait is bounded; a timeout sets the error word, fills the rest of the
 // CTA's tiles with a NaN of its own and drains the pipeline.
 #include "device_common.cuh"

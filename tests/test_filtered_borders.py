@@ -5,8 +5,8 @@ below the distances tested.
 
 Ids and counts are compared exactly.  That is a demand on the kernel only where a
 border is farther away than the kernel's sums are off: 2^-43 of the row's mass.  The
-coins of these rows are multiples of 2^-24, and `far_enough`
-leaves out those that lie closer than that to a border.
+coins of these rows are multiples of 2^-24, and `far_enough` leaves out those that lie
+closer than that to a border.
 """
 import numpy as np
 import pytest

@@ -40,3 +40,15 @@ def test_settings_and_outputs_by_row(pkg, B, logits):
     flags = got["row_flags"].tolist()
     bad = pkg.ROW_NAN | pkg.ROW_NO_CANDIDATE
     assert flags == [bad if B > 4 and b in (3, 4) else 0 for b in range(B)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_norm_of_a_row_whose_squares_overflow(pkg, dtype):
+    """fp32 squares, as in rmsnorm_bf16: 1 / sqrt(infinity) makes the row zeros, and no other row."""
+    x = torch.randn(3, 700, generator=torch.Generator().manual_seed(1)).to(dtype).cuda()
+    x[1] *= 1e20
+    q, s = pkg.rmsnorm_fp8(x, torch.ones(700, device="cuda"))
+    torch.cuda.synchronize()
+    assert not bool(q[1].float().any()) and bool((s[1] == 2.0 ** -126).all())
+    assert bool((q[[0, 2]].float().abs().amax(1) == 448.0).all())

@@ -331,7 +331,7 @@ typedef struct {
  *   out_ids          [batch] token ids; 0 on a row without candidates, which is
  *                    flagged SAMPLER_ROW_NO_CANDIDATE
  *   out_logprobs     [batch] or NULL: ln(w_id / mass of the n), the mass within
- *                    2^-17 relative; -infinity without candidates
+ *                    2^-18 relative; -infinity without candidates
  *   out_kept         [batch] or NULL: n
  *   row_flags        [batch] or NULL: SAMPLER_ROW_NAN, SAMPLER_ROW_NO_CANDIDATE
  * What decides an id is held to about 2^-43 of the row's mass, so ids are those of

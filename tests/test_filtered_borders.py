@@ -344,3 +344,19 @@ def test_finite_masks_with_top_k_and_min_p(pkg):
         check(pkg, y, 0.8, 700, 1.0, 0.01, coins)
         times.append(time_of(pkg, y, (0.8, 700, 1.0, 0.01), c))
     assert times[1] <= 3.0 * times[0], times
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,top", [(0.6, 0.0), (0.8, 40.0), (1.3, -300.0), (1e-2, 1500.3), (1e-5, 812.7), (1e-6, 90000.0)])
+def test_log_probabilities_of_open_rows(pkg, T, top):
+    """ln of the share of an entry of the whole row: the mass within 2^-18, whatever the logits' distance from 0 is
+    against the temperature, and half a step of fp32 for the result."""
+    for V in (300, 32000, 100003):
+        rows = [np.float32(top) + heads_above_a_floor(V, V // 2, T, bits, bits) * np.float32(T if T < 0.1 else 1.0)
+                for bits in (3, 20, 41)]
+        coins = np.array([0.3, 0.6, 0.999], np.float32)
+        got = call(pkg, torch.from_numpy(np.stack(rows)).cuda(), T, 0, 1.0, 0.0, coins)
+        for x, i, lp in zip(rows, got[0], got[1]):
+            row = Row(x, np.float32(T))
+            want = (LD(x[i]) - LD(x.max())) / LD(np.float32(T)) - np.log(row.mass)
+            assert abs(LD(lp) - want) <= LD(2) ** -18 + LD(2) ** -24 * abs(want), (V, float(lp), float(want))
